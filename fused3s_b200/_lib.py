@@ -21,6 +21,7 @@ F3S_ERR_CUDA = 5
 F3S_ERR_TIMEOUT = 6
 F3S_ERR_BAD_FORMAT = 7
 F3S_ERR_TOO_LARGE = 8
+F3S_ERR_NO_PAGES = 9
 
 F3S_IPC_HANDLE_BYTES = 64
 
@@ -33,6 +34,7 @@ _I32 = ctypes.c_int32
 _I64 = ctypes.c_int64
 _SZ = ctypes.c_size_t
 _U64 = ctypes.c_uint64
+_F32 = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/fused3s.h one to one
 SIGNATURES = {
@@ -73,6 +75,18 @@ SIGNATURES = {
     "f3s_1tb1rw_launch": (ctypes.c_int, [_P, _P, _P, _P, _P, _P, _P, _I32, _I32, _P]),
     "f3s_half_from_float": (ctypes.c_int, [_P, _P, _I64, _P]),
     "f3s_selftest_wait_timeout": (ctypes.c_int, [_U64, _P, _SZ, _P]),
+    "f3s_kv4_record_bytes": (_SZ, [_I32]),
+    "f3s_kv4_store": (ctypes.c_int, [_P, _P, _I32, _I64, _I64, _I64, _I64, _P, _I64, _P, _I32, _I32, _I32, _P, _SZ,
+                                     _P]),
+    "f3s_kv4_load": (ctypes.c_int, [_P, _I32, _I32, _I32, _P, _I64, _P, _P, _I32, _P, _SZ, _P]),
+    "f3s_block_tables_workspace_size": (_SZ, [_I32, _I64, _I32, _I32]),
+    "f3s_block_tables": (ctypes.c_int, [_P, _P, _I32, _P, _I64, _I32, _P, _I32, _P, _I64, _I32, _I32, _P, _P, _P, _P,
+                                        _P, _SZ, _P]),
+    "f3s_kv4_attention_workspace_size": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
+    "f3s_kv4_attention": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I32, _P, _I64, _P, _I32, _I64, _I32, _I32,
+                                         _I32, _F32, _P, _I32, _P, _SZ, _P]),
+    "f3s_kv4_forward": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _I32, _P, _P, _P, _I32, _I32, _I32, _I32, _I32, _F32,
+                                       _I32, _I32, _P, _SZ, _P]),
     "f3s_probe_mma_sync": (ctypes.c_int, [_I32, _I32, ctypes.POINTER(ctypes.c_double), _P]),
 }
 

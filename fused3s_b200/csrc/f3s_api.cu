@@ -136,11 +136,12 @@ const char* f3s_status_string(int status) {
         case F3S_ERR_TIMEOUT: return "F3S_ERR_TIMEOUT: a bounded device wait expired";
         case F3S_ERR_BAD_FORMAT: return "F3S_ERR_BAD_FORMAT: window id or block column out of range";
         case F3S_ERR_TOO_LARGE: return "F3S_ERR_TOO_LARGE: exceeds int32 limits of the format";
+        case F3S_ERR_NO_PAGES: return "F3S_ERR_NO_PAGES: the free list holds fewer pages than are needed";
         default: return "F3S_ERR_UNKNOWN";
     }
 }
 
-int f3s_version(void) { return 1 * 10000 + 1 * 100 + 0; }
+int f3s_version(void) { return 1 * 10000 + 2 * 100 + 0; }
 
 int f3s_set_forward_sm_limit(int32_t max_ctas) { return f3s::set_forward_sm_limit(max_ctas); }
 

@@ -48,7 +48,8 @@ typedef enum f3s_status {
     F3S_ERR_CUDA = 5,          /* a CUDA runtime call failed                      */
     F3S_ERR_TIMEOUT = 6,       /* a bounded device-side wait expired              */
     F3S_ERR_BAD_FORMAT = 7,    /* window id / block column outside its range      */
-    F3S_ERR_TOO_LARGE = 8      /* exceeds the int32 limits of the format          */
+    F3S_ERR_TOO_LARGE = 8,     /* exceeds the int32 limits of the format          */
+    F3S_ERR_NO_PAGES = 9       /* the free list holds fewer pages than are needed */
 } f3s_status;
 
 /* Human-readable name of a status code (static storage). */
@@ -403,6 +404,121 @@ int f3s_peer_open(const void* ipc_handle, void** d_ptr);
 int f3s_peer_close(void* d_ptr);
 int f3s_peer_free(void* d_ptr);
 int f3s_peer_copy(void* d_dst, const void* d_src, size_t bytes, f3s_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * K / V held in 4 bits (no reference counterpart: the reference reads fp16).
+ *
+ * A page holds 16 tokens -- the 16 rows of one block column -- of kv_heads
+ * heads: d_pages is uint8[num_pages][kv_heads][16 * head_dim + 128].  The
+ * record of a page and head holds, in this order,
+ *   K codes  8 * head_dim bytes: 32-bit words [16 tokens][head_dim / 8]; bits
+ *            4 n + 16 h ... + 3 of word w are the code of channel 8 w + 2 n + h;
+ *   V codes  8 * head_dim bytes: 16-bit halves [2][8][4][head_dim / 32][2];
+ *            bits 4 n ... + 3 of half (p, g, t, w, l) are the code of channel
+ *            g * head_dim / 8 + 4 w + n of token 8 p + 2 t + l;
+ *   scales   fp16[8][2][2][2]: [token % 8][token / 8][K, V][scale, zero].
+ * A value is scale * (code - zero), code and zero whole numbers 0 ... 15.
+ * A slot is page * 16 + token (int32); -1 means no slot.  Page buffers are
+ * 16-byte aligned and hold at most 2^31 / 16 - 1 pages.
+ *
+ * f3s_kv4_store quantises token i's row of every head into d_slots[i] (rows
+ * of slot -1 are skipped).  Per row x: the scale is the row's range, zero
+ * included, over 15, rounded to fp16 and kept within [2^-24, 65504]; the zero
+ * is round(-min / scale); a code is round(x / scale) + zero, clamped to 0 ...
+ * 15; halves round to even.  A row with a NaN stands for NaN.  Slots have to
+ * differ from each other (of two equal ones no defined mixture is kept).
+ * Inputs are fp16 or bf16 [num_tokens][kv_heads][head_dim] with the given
+ * strides in elements (multiples of 8; head_dim contiguous; 16-byte aligned).
+ * f3s_kv4_load writes the values of the slots' rows to contiguous
+ * [num_tokens][kv_heads][head_dim] tensors of dtype (f3s_out_dtype), rounded
+ * to nearest; rows of slot -1 become 0.  A slot outside the cache (and not
+ * -1) is reported as F3S_ERR_BAD_FORMAT in the workspace and skipped (load: 0).
+ * The workspace of both: f3s_forward_workspace_size() bytes, zeroed once.
+ * ---------------------------------------------------------------------- */
+size_t f3s_kv4_record_bytes(int32_t head_dim);
+int f3s_kv4_store(const void* d_K, const void* d_V, int32_t dtype, int64_t k_token_stride, int64_t k_head_stride,
+                  int64_t v_token_stride, int64_t v_head_stride, const int32_t* d_slots, int64_t num_tokens,
+                  void* d_pages, int32_t num_pages, int32_t kv_heads, int32_t head_dim, void* d_workspace,
+                  size_t workspace_bytes, f3s_stream_t stream);
+int f3s_kv4_load(const void* d_pages, int32_t num_pages, int32_t kv_heads, int32_t head_dim, const int32_t* d_slots,
+                 int64_t num_tokens, void* d_K, void* d_V, int32_t dtype, void* d_workspace, size_t workspace_bytes,
+                 f3s_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Block tables, slot maps and the attention plan from request lengths (no
+ * reference counterpart; the request-side f3s_convert: a table row lists a
+ * request's block columns).
+ *
+ * Request i has d_context_lens[i] tokens in the cache and d_new_lens[i] new
+ * ones.  Row i of d_tables (int32, table_width entries, rows table_stride
+ * apart) holds its ceil(context / 16) pages so far; the call appends the
+ * pages that the new tokens need, taken in request order from
+ * d_free_pages[*d_free_begin ...] (NULL: from 0), and writes
+ *   d_query_offsets[num_requests + 1]  first new token of each request
+ *   d_positions[num_tokens]            position of each new token in its request
+ *   d_slots[num_tokens]                its slot (table entry * 16 + position % 16)
+ *   d_free_begin_out[1]                the first page that is still free
+ * (d_free_begin_out may be d_free_begin's memory only for a call that is not
+ * repeated.)  num_tokens is the capacity of the token arrays; entries behind
+ * the last new token get slot -1 and position 0.
+ * heads, kv_heads: attention heads the plan is made for (0, 0: no plan).
+ * d_plan: f3s_block_tables_workspace_size bytes, 16-byte aligned, also this
+ * call's workspace (f3s_workspace_status); the call sets its status:
+ *   F3S_ERR_NO_PAGES       the free list is too short; the tokens without a
+ *                          page get slot -1 and their table entries -1
+ *   F3S_ERR_TOO_LARGE      more new tokens than num_tokens, or a request that
+ *                          is longer than its table row; what does not fit
+ *                          has slot -1 (or no entry) and is not attended
+ *   F3S_ERR_INVALID_VALUE  a negative length, taken as 0
+ * ---------------------------------------------------------------------- */
+size_t f3s_block_tables_workspace_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads);
+int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, int32_t num_requests, int32_t* d_tables,
+                     int64_t table_stride, int32_t table_width, const int32_t* d_free_pages, int32_t num_free,
+                     const int32_t* d_free_begin, int64_t num_tokens, int32_t heads, int32_t kv_heads,
+                     int32_t* d_query_offsets, int32_t* d_positions, int32_t* d_slots, int32_t* d_free_begin_out,
+                     void* d_plan, size_t plan_bytes, f3s_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Causal attention of the new tokens over a 4-bit cache (no reference
+ * counterpart).
+ *
+ * The new token at position p of its request attends to the request's
+ * positions 0 ... p (its own K / V stored before this call):
+ *   O[i, h, :] = sum_t softmax_t(scale * Q[i, h, :] . K[t, g, :]) V[t, g, :]
+ * with K/V head g = h / (heads / kv_heads).
+ *   d_Q      fp16 or bf16 [num_tokens][heads][head_dim], strides in elements
+ *            (multiples of 8; head_dim contiguous; 16-byte aligned)
+ *   d_O      contiguous [num_tokens][heads][head_dim] of o_dtype; rows behind
+ *            the last new token are not written
+ *   d_tables, table_stride, num_requests, num_tokens, heads, kv_heads: those that the plan was made with; d_plan is not changed but for
+ *            its status, so several calls may share it
+ *   d_workspace: f3s_kv4_attention_workspace_size bytes, 16-byte aligned, not
+ *            shared by calls that may overlap; needs no initialisation
+ * A table entry of -1 holds no tokens (they are left out); one outside the
+ * cache is too, and is reported as F3S_ERR_BAD_FORMAT in the plan's status.
+ * fp16 and fp32 O are exact to fp32 arithmetic, bf16 O rounds the softmax
+ * weights to fp16.
+ * ---------------------------------------------------------------------- */
+size_t f3s_kv4_attention_workspace_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
+                                        int32_t head_dim);
+int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, int64_t q_head_stride,
+                      const void* d_pages, int32_t num_pages, const int32_t* d_tables, int64_t table_stride,
+                      void* d_plan, int32_t num_requests, int64_t num_tokens, int32_t heads,
+                      int32_t kv_heads, int32_t head_dim, float scale, void* d_O, int32_t o_dtype, void* d_workspace,
+                      size_t workspace_bytes, f3s_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * f3s_forward over K / V held in 4 bits: block column c of the format is page
+ * c of d_pages (node v is slot v), columns >= num_nodes are masked.  Scores
+ * are multiplied by `scale` (f3s_forward: 1); query head h reads K/V head
+ * h / (heads / kv_heads); Q is contiguous fp16 or bf16.  Other arguments,
+ * window lists and slabs as f3s_forward_ex.  num_pages >= ceil(num_nodes / 16).
+ * ---------------------------------------------------------------------- */
+int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32_t num_pages, void* d_O,
+                    int32_t o_dtype, const int32_t* d_window_offsets, const int32_t* d_block_cols,
+                    const int32_t* d_order, int32_t num_items, int32_t num_nodes, int32_t heads, int32_t kv_heads,
+                    int32_t head_dim, float scale, int32_t q_window_base, int32_t q_rows, void* d_workspace,
+                    size_t workspace_bytes, f3s_stream_t stream);
 
 #ifdef __cplusplus
 }
