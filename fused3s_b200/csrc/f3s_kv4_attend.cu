@@ -34,6 +34,8 @@ constexpr uint64_t kAttendTimeoutNs = 5ull * 1000 * 1000 * 1000;
 constexpr float kNoReference = -3.0e38f;  // finite: a weight against it is 0, not NaN
 constexpr float kRescaleAt = 8.f;
 
+struct WindowPieces;
+
 struct AttendParams {
     const void* q;
     int64_t q_token, q_head;  // strides in elements
@@ -51,19 +53,125 @@ struct AttendParams {
     const int* tables;
     int64_t table_stride;
     // windows
+    WindowPieces* pieces;
+    const int4* heavy_items;
+    const int* light_items;
+    const int4* window_splits;
+    int heavy_cap, splits_cap;
     const int* offsets;
     const int* cols;
-    const int* order;
-    int num_items;
     int num_nodes, windows, q_window_base, q_rows;
-    int warps_per_unit;  // 4, or 1: one warp per window and head
 };
+
+// The windows of a graph as work for warps and blocks (k_window_pieces).
+// A window of at most `light` blocks is one warp's, per head; a heavier one
+// is cut into pieces of at most `heavy` blocks, each a block's of four warps,
+// and a window of several pieces has their sums merged.
+struct WindowPieces {
+    int heavy_items, light_items, splits, slots;
+    int heavy_ticket, light_ticket;
+    int pad[58];
+};
+static_assert(sizeof(WindowPieces) == 256, "piece header is 256 bytes");
+
+struct WindowPieceLayout {
+    int light, heavy;
+    int64_t heavy_cap, splits_cap, slots_cap;
+    size_t heavy_items, light_items, splits, partials, total;
+};
+
+// A light window holds at most a quarter of a warp's even share of the work
+// (and 8 blocks are one warp's in any case), a piece at most four times that.
+static WindowPieceLayout window_piece_layout(int num_items, int64_t num_blocks, int heads, int head_dim, int sms) {
+    WindowPieceLayout L{};
+    const int64_t warps = (int64_t)sms * 16;
+    const int64_t share = (num_blocks * heads + 4 * warps - 1) / (4 * warps);
+    L.light = (int)std::min<int64_t>(std::max<int64_t>(share, 8), 1 << 28);
+    L.heavy = 4 * L.light;
+    const int64_t cut = num_blocks / L.heavy;
+    L.heavy_cap = std::min<int64_t>(num_items, num_blocks / L.light) + cut;
+    L.splits_cap = std::min<int64_t>(num_items, cut);
+    L.slots_cap = 2 * cut;
+    size_t off = sizeof(WindowPieces);
+    L.heavy_items = off;
+    off += (size_t)L.heavy_cap * 16;
+    L.splits = off;
+    off += (size_t)L.splits_cap * 16;
+    L.light_items = off;
+    off = align_up(off + (size_t)num_items * 4, 16);
+    L.partials = off;
+    off += (size_t)L.slots_cap * heads * 16 * (head_dim + 2) * 4;
+    L.total = off;
+    return L;
+}
+
+struct WindowPieceParams {
+    const int* offsets;
+    const int* order;
+    int num_items, windows, q_window_base, q_rows;
+    int light, heavy, heavy_cap, splits_cap, slots_cap;
+    WindowPieces* pieces;
+    int4* heavy_items;  // window, first block, end block, slot or -1
+    int* light_items;
+    int4* splits;       // window, first slot, pieces, -
+    int* status;
+};
+
+// One thread per listed window.  Blocks reserve their share of the lists with
+// atomics, so the lists' order varies; a window's cuts and the order in which
+// its pieces are summed do not.
+__global__ void __launch_bounds__(256) k_window_pieces(const WindowPieceParams p) {
+    __shared__ int s_scan[256 / 32 + 1], s_base[4];
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    int window = 0, b0 = 0, nb = 0;
+    bool live = i < p.num_items;
+    if (live) {
+        window = p.order[i];
+        live = window >= p.q_window_base && window < p.windows && (int64_t)(window - p.q_window_base) * 16 < p.q_rows;
+        if (!live) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
+    }
+    if (live) {
+        b0 = p.offsets[window];
+        nb = max(p.offsets[window + 1] - b0, 0);
+    }
+    const bool heavy = live && nb > p.light;
+    const int parts = heavy ? (int)(((int64_t)nb + p.heavy - 1) / p.heavy) : 0;
+    const bool split = parts > 1;
+    int total[4], at[4];
+    at[0] = block_exclusive_scan<256>(parts, total[0], s_scan);
+    at[1] = block_exclusive_scan<256>(live && !heavy, total[1], s_scan);
+    at[2] = block_exclusive_scan<256>(split, total[2], s_scan);
+    at[3] = block_exclusive_scan<256>(split ? parts : 0, total[3], s_scan);
+    if (threadIdx.x < 4) {
+        int* counters[4] = {&p.pieces->heavy_items, &p.pieces->light_items, &p.pieces->splits, &p.pieces->slots};
+        s_base[threadIdx.x] = atomicAdd(counters[threadIdx.x], total[threadIdx.x]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; ++k) at[k] += s_base[k];
+    if (live && !heavy) p.light_items[at[1]] = window;
+    // more blocks than the caller said (a heavy window listed many times): one
+    // warp takes what the lists have no room for
+    if (heavy && (at[0] + parts > p.heavy_cap || (split && (at[2] >= p.splits_cap || at[3] + parts > p.slots_cap)))) {
+        for (int k = 0; k < parts && at[0] + k < p.heavy_cap; ++k) p.heavy_items[at[0] + k] = make_int4(-1, 0, 0, -1);
+        if (split && at[2] < p.splits_cap) p.splits[at[2]] = make_int4(-1, 0, 0, 0);
+        p.light_items[atomicAdd(&p.pieces->light_items, 1)] = window;
+        return;
+    }
+    for (int k = 0; k < parts; ++k) {
+        const int lo = (int)((int64_t)nb * k / parts), hi = (int)((int64_t)nb * (k + 1) / parts);
+        p.heavy_items[at[0] + k] = make_int4(window, b0 + lo, b0 + hi, split ? at[3] + k : -1);
+    }
+    if (split) p.splits[at[2]] = make_int4(window, at[3], parts, 0);
+}
 
 template <int D, int NT>
 struct AttendCfg {
     static constexpr int RB = kv4_record_bytes(D);
-    static constexpr int STAGES = D == 64 ? 8 : 4;
-    static constexpr int RING = kAttendWarps * STAGES * RB;
+    static constexpr int PP = NT == 4 ? 1 : 2;  // pages per step and stage
+    static constexpr int STAGES = (D == 64 ? 8 : 4) / PP;
+    static constexpr int STAGE_BYTES = PP * RB;
+    static constexpr int RING = kAttendWarps * STAGES * STAGE_BYTES;
     static constexpr bool Q_SMEM = NT == 4;  // four warps per unit only: they share it
     static constexpr int Q_BYTES = Q_SMEM ? 8 * NT * D * 2 : 0;
     static constexpr int OPITCH = D + 4;
@@ -96,6 +204,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ float log2_approx(float x) {
     float y;
     asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -154,22 +268,41 @@ __device__ __forceinline__ void store_channels(void* o, int64_t idx, const float
     for (int i = 0; i < CH / 8; ++i) __stcs(dst + i, make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
 }
 
+// 2 or 4 values, as above.
+template <int E>
+__device__ __forceinline__ void store_few(void* o, int64_t idx, const float (&v)[E], int dtype) {
+    if (dtype == F3S_OUT_F32) {
+        float* dst = static_cast<float*>(o) + idx;
+        if constexpr (E == 4) __stcs(reinterpret_cast<float4*>(dst), make_float4(v[0], v[1], v[2], v[3]));
+        else __stcs(reinterpret_cast<float2*>(dst), make_float2(v[0], v[1]));
+        return;
+    }
+    uint32_t w[E / 2];
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) {
+        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = dtype == F3S_OUT_F16 ? pack_half2(v[2 * i], v[2 * i + 1]) : *reinterpret_cast<const uint32_t*>(&b);
+    }
+    uint16_t* dst = static_cast<uint16_t*>(o) + idx;
+    if constexpr (E == 4) __stcs(reinterpret_cast<uint2*>(dst), make_uint2(w[0], w[1]));
+    else __stcs(reinterpret_cast<unsigned int*>(dst), w[0]);
+}
+
 // PAGED: a unit is (work item of the plan, K/V head) and the CTA's four warps
-// take its pages in turn.  Otherwise a unit is (window, head): four warps in
-// turn, or one warp.  PRECISE adds the part of P that rounding to fp16 drops
+// take its pages in turn.  Otherwise persistent CTAs take units by ticket: first
+// (piece, head), four warps in turn, then each warp (light window, head) by
+// itself; the next ticket is drawn while a unit runs.  PRECISE adds the part of P that rounding to fp16 drops
 // with a second product, which makes the result as exact as fp32 arithmetic.
 template <int D, int NT, bool PAGED, bool PRECISE>
 __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS) k_attend4(const AttendParams p) {
     using C = AttendCfg<D, NT>;
-    constexpr int RB = C::RB, STAGES = C::STAGES;
+    constexpr int RB = C::RB, STAGES = C::STAGES, PP = C::PP;
     constexpr int W = D / 32;    // words of a token's K (and of a token pair's V) per lane
     constexpr int CH = D / 8;    // output channels per lane
     constexpr int TQ = 8 * NT;   // query rows of a tile
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int wpu = PAGED ? kAttendWarps : p.warps_per_unit;
-    const int wq = wpu == 1 ? 0 : warp;
-    uint8_t* ring = smem + warp * STAGES * RB;
+    uint8_t* ring = smem + warp * STAGES * C::STAGE_BYTES;
     const uint32_t ring_a = smem_addr(ring);
     const uint32_t bars = smem_addr(smem + C::BARS) + warp * STAGES * 8;
     const uint32_t sink = smem_addr(smem + C::SINK) + warp * 4;
@@ -180,19 +313,48 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     }
     __syncwarp();
     bool dead = false;  // a wait ran out: no more pages for this warp
-    uint32_t used = 0;  // pages this warp has streamed: stage and parity of the next
+    uint32_t used = 0;  // steps this warp has streamed: stage and parity of the next
 
-    const int per_cta = kAttendWarps / wpu;
     const int kv_units = PAGED ? p.kv_heads : p.heads;
-    const int64_t units = (int64_t)(PAGED ? p.plan->num_items : p.num_items) * kv_units;
     const int64_t page_bytes = (int64_t)p.kv_heads * RB;
+    int wpu = kAttendWarps, wq = warp;  // warps per unit, this one among them
+    int64_t units, light_units = 0;
+    int ticket = 0;
+    __shared__ int s_ticket;
+    if constexpr (PAGED) {
+        units = (int64_t)p.plan->num_items * kv_units;
+    } else {
+        units = (int64_t)min(p.pieces->heavy_items, p.heavy_cap) * kv_units;
+        light_units = (int64_t)p.pieces->light_items * kv_units;
+        if (threadIdx.x == 0) ticket = atomicAdd(&p.pieces->heavy_ticket, 1);
+    }
 
-    for (int64_t base = (int64_t)blockIdx.x * per_cta; base < units; base += (int64_t)gridDim.x * per_cta) {
-        const int64_t unit = base + (wpu == 1 ? warp : 0);
-        if (unit >= units) break;  // one warp per unit: nothing is shared
+    for (int64_t unit = blockIdx.x;; unit += gridDim.x) {
+        if constexpr (PAGED) {
+            if (unit >= units) break;
+        } else {
+            if (wpu == kAttendWarps) {
+                if (threadIdx.x == 0) s_ticket = ticket;
+                __syncthreads();
+                unit = s_ticket;
+                if (unit >= units) {  // for every warp of the CTA
+                    wpu = 1;
+                    wq = 0;
+                    if (lane == 0) ticket = atomicAdd(&p.pieces->light_ticket, 1);
+                } else if (threadIdx.x == 0) {
+                    ticket = atomicAdd(&p.pieces->heavy_ticket, 1);
+                }
+            }
+            if (wpu == 1) {
+                unit = __shfl_sync(0xffffffffu, ticket, 0);
+                if (unit >= light_units) break;
+                if (lane == 0) ticket = atomicAdd(&p.pieces->light_ticket, 1);
+            }
+        }
         const int item = (int)(unit / kv_units), sub = (int)(unit - (int64_t)item * kv_units);
         const int hk = PAGED ? sub : sub / p.group;
         Kv4Item it{};
+        it.slot = -1;
         const int* list;
         int first, count;  // blocks of the unit
         int window = 0;
@@ -211,18 +373,27 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             first = it.page0;
             count = max(it.page1 - it.page0, 0);
         } else {
-            window = p.order[item];
-            const bool ok = window >= p.q_window_base && window < p.windows &&
-                            (int64_t)(window - p.q_window_base) * 16 < p.q_rows;
-            if (!ok) {
-                if (lane == 0) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
-                continue;  // the whole unit: every warp of it sees the same window
-            }
             list = p.cols;
-            first = p.offsets[window];
-            count = max(p.offsets[window + 1] - first, 0);
+            if (wpu == 1) {
+                window = p.light_items[item];
+                first = p.offsets[window];
+                count = max(p.offsets[window + 1] - first, 0);
+            } else {
+                const int4 piece = __ldcg(p.heavy_items + item);
+                window = piece.x;
+                first = piece.y;
+                count = piece.z - piece.y;
+                it.slot = piece.w;
+                if (window < 0) {  // did not fit the lists
+                    __syncthreads();
+                    continue;
+                }
+            }
         }
-        const int own = !dead && count > wq ? (count - wq + wpu - 1) / wpu : 0;
+        // this warp's pages: PP in a row of every PP * wpu
+        const int mine = dead ? 0 : count - wq * PP;
+        const int steps = mine > 0 ? (mine + PP * wpu - 1) / (PP * wpu) : 0;
+        const int own = steps ? (steps - 1) * PP + min(PP, mine - (steps - 1) * PP * wpu) : 0;
         const int limit_id = PAGED ? p.num_pages : p.windows;
 
         // ---- page ids, 32 at a time (one per lane), the next 32 ahead
@@ -230,7 +401,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             const int i = batch * 32 + lane;
             int id = 0;
             if (i < own) {
-                id = __ldg(list + first + wq + (int64_t)i * wpu);
+                id = __ldg(list + first + wq * PP + (int64_t)(i / PP) * PP * wpu + i % PP);
                 if (id < 0 || id >= limit_id) {
                     if (!(PAGED && id == -1)) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
                     id = -1;
@@ -240,23 +411,32 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         };
         int ids = load_ids(0), ids_next = 0;
         uint32_t skip = 0, tail = 0;  // of the pages in flight, bit (page index % 32)
-        auto issue = [&](int i) {
+        auto issue = [&](int step) {
+            const int i = step * PP;
             if ((i & 31) == 0) {
                 if (i > 0) ids = ids_next;
                 if (i + 32 < own) ids_next = load_ids(i / 32 + 1);
             }
-            const int id = __shfl_sync(0xffffffffu, ids, i & 31);
-            const uint32_t bit = 1u << (i & 31);
-            skip = id < 0 ? skip | bit : skip & ~bit;
-            if constexpr (!PAGED) tail = id == p.windows - 1 ? tail | bit : tail & ~bit;
-            const uint32_t n = used + i, st = n % STAGES;
+            int id[PP];
+#pragma unroll
+            for (int k = 0; k < PP; ++k) {
+                id[k] = __shfl_sync(0xffffffffu, ids, (i + k) & 31);
+                const uint32_t bit = 1u << ((i + k) & 31);
+                skip = id[k] < 0 || i + k >= own ? skip | bit : skip & ~bit;
+                if constexpr (!PAGED) tail = id[k] == p.windows - 1 ? tail | bit : tail & ~bit;
+            }
+            const uint32_t n = used + step, st = n % STAGES;
             if (lane == 0) {
-                mbar_arrive_expect_tx(bars + 8 * st, RB);
-                bulk_load(ring_a + st * RB, p.pages + (int64_t)max(id, 0) * page_bytes + (int64_t)hk * RB, RB,
-                          bars + 8 * st);
+                const int have = min(PP, own - i);
+                mbar_arrive_expect_tx(bars + 8 * st, have * RB);
+#pragma unroll
+                for (int k = 0; k < PP; ++k)
+                    if (k < have)
+                        bulk_load(ring_a + st * C::STAGE_BYTES + k * RB,
+                                  p.pages + (int64_t)max(id[k], 0) * page_bytes + (int64_t)hk * RB, RB, bars + 8 * st);
             }
         };
-        for (int i = 0; i < min(own, STAGES); ++i) issue(i);
+        for (int i = 0; i < min(steps, STAGES); ++i) issue(i);
 
         // ---- Q: rows g of each n-tile, channels t * D / 4 ..., as fp16 times a
         // power of two that brings the tile's largest to [2^9, 2^10); channels
@@ -373,7 +553,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         // first token that some row of the tile must not see
         const int open = PAGED ? it.context + it.row0 / p.group + 1 : 0;
 
-        for (int i = 0; i < own; ++i) {
+        for (int i = 0; i < steps; ++i) {
             const uint32_t n = used + i, st = n % STAGES, parity = (n / STAGES) & 1;
             bool ready = mbar_try_wait(bars + 8 * st, parity);
             if (!__all_sync(0xffffffffu, ready)) {
@@ -383,97 +563,108 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                     break;
                 }
             }
-            const uint8_t* rec = ring + st * RB;
-            // ---- S^T = K Q^T
-            uint32_t kg[W], kh[W], v0[W], v1[W];
-            lds_words<W>(rec + g * (D / 2) + t * (D / 8), kg);
-            lds_words<W>(rec + (g + 8) * (D / 2) + t * (D / 8), kh);
-            const uint4 sc = *reinterpret_cast<const uint4*>(rec + 16 * D + g * 16);
-            lds_words<W>(rec + 8 * D + lane * (D / 8), v0);
-            lds_words<W>(rec + 12 * D + lane * (D / 8), v1);
-            float s[NT][2][4];
+            uint32_t dep = 0;
+            float x[PP][NT][4];
+            float ri[PP][2], vz[PP][2];  // 1 / r and y of tokens g, g + 8
+            const uint8_t* rec0 = ring + st * C::STAGE_BYTES;
 #pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const uint32_t a8 = kg[w] >> 8, b8 = kh[w] >> 8;
-                const uint32_t a0[4] = {kg[w] & kNib0, kh[w] & kNib0, kg[w] & kNib1, kh[w] & kNib1};
-                const uint32_t a1[4] = {a8 & kNib0, b8 & kNib0, a8 & kNib1, b8 & kNib1};
+            for (int k = 0; k < PP; ++k) {
+                // ---- S^T = K Q^T
+                const uint8_t* rec = rec0 + k * RB;
+                uint32_t kg[W], kh[W];
+                lds_words<W>(rec + g * (D / 2) + t * (D / 8), kg);
+                lds_words<W>(rec + (g + 8) * (D / 2) + t * (D / 8), kh);
+                const uint4 sc = *reinterpret_cast<const uint4*>(rec + 16 * D + g * 16);
+                dep ^= kg[0] ^ kh[0] ^ sc.x;
+                float s[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    uint32_t b[4];
-                    if constexpr (C::Q_SMEM) {
-                        const uint4 x = qsm[(nt * W + w) * 32 + lane];
-                        b[0] = x.x;
-                        b[1] = x.y;
-                        b[2] = x.z;
-                        b[3] = x.w;
-                    } else {
+                for (int w = 0; w < W; ++w) {
+                    const uint32_t a8 = kg[w] >> 8, b8 = kh[w] >> 8;
+                    const uint32_t a0[4] = {kg[w] & kNib0, kh[w] & kNib0, kg[w] & kNib1, kh[w] & kNib1};
+                    const uint32_t a1[4] = {a8 & kNib0, b8 & kNib0, a8 & kNib1, b8 & kNib1};
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) b[n] = qf[nt][w][n];
-                    }
-                    constexpr int odd = NT == 1 ? 1 : 0;  // one n-tile: two chains
-                    if (w == 0) {
-                        mma_16816_zero(s[nt][0], a0, b[0], b[1]);
-                        if (odd) mma_16816_zero(s[nt][1], a1, b[2], b[3]);
-                        else mma_16816(s[nt][0], a1, b[2], b[3]);
-                    } else {
-                        mma_16816(s[nt][0], a0, b[0], b[1]);
-                        mma_16816(s[nt][odd], a1, b[2], b[3]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        uint32_t b[4];
+                        if constexpr (C::Q_SMEM) {
+                            const uint4 y = qsm[(nt * W + w) * 32 + lane];
+                            b[0] = y.x;
+                            b[1] = y.y;
+                            b[2] = y.z;
+                            b[3] = y.w;
+                        } else {
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) b[m] = qf[nt][w][m];
+                        }
+                        if (w == 0) mma_16816_zero(s[nt], a0, b[0], b[1]);
+                        else mma_16816(s[nt], a0, b[0], b[1]);
+                        mma_16816(s[nt], a1, b[2], b[3]);
                     }
                 }
-            }
-            // ---- scores to weights
-            const float2 ka = __half22float2(*reinterpret_cast<const __half2*>(&sc.x));
-            const float2 va = __half22float2(*reinterpret_cast<const __half2*>(&sc.y));
-            const float2 kb = __half22float2(*reinterpret_cast<const __half2*>(&sc.z));
-            const float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&sc.w));
-            const float fa = ka.x * 1048576.f * unit_scale, fb = kb.x * 1048576.f * unit_scale;  // 2^20: the codes' unit
-            const float ra = va.x < kKv4MinScale ? kKv4MinScale : va.x;  // keeps a NaN
-            const float rb = vb.x < kKv4MinScale ? kKv4MinScale : vb.x;
-            const float la = log2_approx(ra), lb = log2_approx(rb);
-            const float ia = __frcp_rn(ra), ib = __frcp_rn(rb);
-            const int tok0 = PAGED ? (it.page0 + wq + i * wpu) * 16 : 0;
-            const bool skipped = (skip >> (i & 31)) & 1;
-            bool masked;
-            if constexpr (PAGED) masked = skipped || tok0 + 16 > open;
-            else masked = skipped || ((tail >> (i & 31)) & 1);
-            float x[NT][4];
-            bool over = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    float d = s[nt][0][c];
-                    if (NT == 1) d += s[nt][1][c];
-                    const float z = c < 2 ? ka.y : kb.y;
-                    x[nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], d), c < 2 ? fa : fb, c < 2 ? la : lb);
-                }
-            if (masked) {
+                // ---- scores
+                const float2 ka = __half22float2(*reinterpret_cast<const __half2*>(&sc.x));
+                const float2 va = __half22float2(*reinterpret_cast<const __half2*>(&sc.y));
+                const float2 kb = __half22float2(*reinterpret_cast<const __half2*>(&sc.z));
+                const float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&sc.w));
+                const float fa = ka.x * 1048576.f * unit_scale, fb = kb.x * 1048576.f * unit_scale;  // 2^20: the codes' unit
+                const float ra = va.x < kKv4MinScale ? kKv4MinScale : va.x;  // keeps a NaN
+                const float rb = vb.x < kKv4MinScale ? kKv4MinScale : vb.x;
+                const float la = log2_approx(ra), lb = log2_approx(rb);
+                ri[k][0] = rcp_approx(ra);
+                ri[k][1] = rcp_approx(rb);
+                vz[k][0] = va.y;
+                vz[k][1] = vb.y;
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        const int tk = g + (c < 2 ? 0 : 8);
-                        bool hide;
-                        if constexpr (PAGED) {
-                            // a tile's rows past its last see what the last sees
-                            const int row = min(it.row0 + nt * 8 + 2 * t + (c & 1), it.rows - 1);
-                            hide = tok0 + tk > it.context + row / p.group;
-                        } else {
-                            hide = (p.windows - 1) * 16 + tk >= p.num_nodes;
-                        }
-                        if (hide || skipped) x[nt][c] = -INFINITY;
+                        const float z = c < 2 ? ka.y : kb.y;
+                        x[k][nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], s[nt][c]), c < 2 ? fa : fb, c < 2 ? la : lb);
                     }
             }
+            // ---- masks: only where a page has tokens that some row must not see
+            const int page = i * PP;  // of this warp's pages
+            const int tok0 = PAGED ? (it.page0 + wq * PP + i * PP * wpu) * 16 : 0;
+            const uint32_t pages_bits = (PP == 2 ? 3u : 1u) << (page & 31);
+            bool masked;
+            if constexpr (PAGED) masked = (skip & pages_bits) || tok0 + 16 * PP > open;
+            else masked = (skip | tail) & pages_bits;
+            if (masked) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int k = 0; k < PP; ++k) {
+                    const bool skipped = (skip >> ((page + k) & 31)) & 1;
+                    const bool last = (tail >> ((page + k) & 31)) & 1;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) over |= x[nt][c] > ref[nt][c & 1] + kRescaleAt;
-            if (__any_sync(0xffffffffu, over)) {
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int tk = g + (c < 2 ? 0 : 8);
+                            bool hide;
+                            if constexpr (PAGED) {
+                                // a tile's rows past its last see what the last sees
+                                const int row = min(it.row0 + nt * 8 + 2 * t + (c & 1), it.rows - 1);
+                                hide = tok0 + 16 * k + tk > it.context + row / p.group;
+                            } else {
+                                hide = last && (p.windows - 1) * 16 + tk >= p.num_nodes;
+                            }
+                            if (hide || skipped) x[k][nt][c] = -INFINITY;
+                        }
+                }
+            }
+            // ---- weights
+            float most = -INFINITY;
+#pragma unroll
+            for (int k = 0; k < PP; ++k)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) most = fmaxf(most, x[k][nt][c] - ref[nt][c & 1]);
+            if (__any_sync(0xffffffffu, most > kRescaleAt)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        float m = fmaxf(x[nt][j], x[nt][j + 2]);
+                        float m = fmaxf(x[0][nt][j], x[0][nt][j + 2]);
+                        if (PP == 2) m = fmaxf(m, fmaxf(x[PP - 1][nt][j], x[PP - 1][nt][j + 2]));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                         m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -483,75 +674,82 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                         den[nt][j] *= c;
                         off[nt][j] *= c;
 #pragma unroll
-                        for (int k = 0; k < D / 16; ++k) {
-                            acc[nt][k][j] *= c;
-                            acc[nt][k][j + 2] *= c;
+                        for (int e = 0; e < D / 16; ++e) {
+                            acc[nt][e][j] *= c;
+                            acc[nt][e][j + 2] *= c;
                         }
                     }
             }
-            uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float a[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) a[c] = exp2_approx(x[nt][c] - ref[nt][c & 1]);
-                const uint32_t h0 = pack_half2(a[0], a[1]), h1 = pack_half2(a[2], a[3]);
-                const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                pb[nt][0] = movmatrix_t(h0);
-                pb[nt][1] = movmatrix_t(h1);
-                if constexpr (PRECISE) {
-                    pl[nt][0] = movmatrix_t(pack_half2(a[0] - r0.x, a[1] - r0.y));
-                    pl[nt][1] = movmatrix_t(pack_half2(a[2] - r1.x, a[3] - r1.y));
-                } else {
-                    // the sums take the weights that the product takes
-                    a[0] = r0.x;
-                    a[1] = r0.y;
-                    a[2] = r1.x;
-                    a[3] = r1.y;
-                }
-                if (masked) {
-                    // a masked token's scale and zero may be anything, NaN too
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const bool on = x[nt][c] != -INFINITY;
-                        den[nt][c & 1] += on ? a[c] * (c < 2 ? ia : ib) : 0.f;
-                        off[nt][c & 1] += on ? a[c] * (c < 2 ? va.y : vb.y) : 0.f;
-                    }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        den[nt][c & 1] = fmaf(a[c], c < 2 ? ia : ib, den[nt][c & 1]);
-                        off[nt][c & 1] = fmaf(a[c], c < 2 ? va.y : vb.y, off[nt][c & 1]);
-                    }
-                }
-            }
-            // ---- O^T += V^T P^T
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const uint32_t a8 = v0[w] >> 8, b8 = v1[w] >> 8;
-                const uint32_t a0[4] = {v0[w] & kNib0, v0[w] & kNib1, v1[w] & kNib0, v1[w] & kNib1};
-                const uint32_t a1[4] = {a8 & kNib0, a8 & kNib1, b8 & kNib0, b8 & kNib1};
+            for (int k = 0; k < PP; ++k) {
+                uint32_t pb[NT][2], pl[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    mma_16816(acc[nt][2 * w], a0, pb[nt][0], pb[nt][1]);
-                    mma_16816(acc[nt][2 * w + 1], a1, pb[nt][0], pb[nt][1]);
+                    float a[4];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) a[c] = exp2_approx(x[k][nt][c] - ref[nt][c & 1]);
+                    const uint32_t h0 = pack_half2(a[0], a[1]), h1 = pack_half2(a[2], a[3]);
+                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                    const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                    pb[nt][0] = movmatrix_t(h0);
+                    pb[nt][1] = movmatrix_t(h1);
                     if constexpr (PRECISE) {
-                        mma_16816(acc[nt][2 * w], a0, pl[nt][0], pl[nt][1]);
-                        mma_16816(acc[nt][2 * w + 1], a1, pl[nt][0], pl[nt][1]);
+                        pl[nt][0] = movmatrix_t(pack_half2(a[0] - r0.x, a[1] - r0.y));
+                        pl[nt][1] = movmatrix_t(pack_half2(a[2] - r1.x, a[3] - r1.y));
+                    } else {
+                        // the sums take the weights that the product takes
+                        a[0] = r0.x;
+                        a[1] = r0.y;
+                        a[2] = r1.x;
+                        a[3] = r1.y;
+                    }
+                    if (masked) {
+                        // a masked token's scale and zero may be anything, NaN too
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const bool on = x[k][nt][c] != -INFINITY;
+                            den[nt][c & 1] += on ? a[c] * ri[k][c / 2] : 0.f;
+                            off[nt][c & 1] += on ? a[c] * vz[k][c / 2] : 0.f;
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            den[nt][c & 1] = fmaf(a[c], ri[k][c / 2], den[nt][c & 1]);
+                            off[nt][c & 1] = fmaf(a[c], vz[k][c / 2], off[nt][c & 1]);
+                        }
+                    }
+                }
+                // ---- O^T += V^T P^T
+                const uint8_t* rec = rec0 + k * RB;
+                uint32_t v0[W], v1[W];
+                lds_words<W>(rec + 8 * D + lane * (D / 8), v0);
+                lds_words<W>(rec + 12 * D + lane * (D / 8), v1);
+                dep ^= v0[0] ^ v1[0];
+#pragma unroll
+                for (int w = 0; w < W; ++w) {
+                    const uint32_t a8 = v0[w] >> 8, b8 = v1[w] >> 8;
+                    const uint32_t a0[4] = {v0[w] & kNib0, v0[w] & kNib1, v1[w] & kNib0, v1[w] & kNib1};
+                    const uint32_t a1[4] = {a8 & kNib0, a8 & kNib1, b8 & kNib0, b8 & kNib1};
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816(acc[nt][2 * w], a0, pb[nt][0], pb[nt][1]);
+                        mma_16816(acc[nt][2 * w + 1], a1, pb[nt][0], pb[nt][1]);
+                        if constexpr (PRECISE) {
+                            mma_16816(acc[nt][2 * w], a0, pl[nt][0], pl[nt][1]);
+                            mma_16816(acc[nt][2 * w + 1], a1, pl[nt][0], pl[nt][1]);
+                        }
                     }
                 }
             }
             // refill the stage once the loads from it have landed in every lane:
             // the store needs a word of each load, and comes before the copy
-            if (i + STAGES < own) {
-                const uint32_t dep = kg[0] ^ kh[0] ^ v0[0] ^ v1[0] ^ sc.x;
+            if (i + STAGES < steps) {
                 asm volatile("st.shared.b32 [%0], %1;" ::"r"(sink), "r"(dep) : "memory");
                 __syncwarp();
                 issue(i + STAGES);
             }
         }
-        used += own;
+        used += steps;
 
         // ---- sums over the tokens of the other lanes; units of the accumulators
 #pragma unroll
@@ -633,8 +831,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) v[k] = fmaf(c, src[k], v[k]);
             }
-            if (PAGED && it.slot >= 0) {
-                float* part = p.partials + ((int64_t)it.slot * p.kv_heads + hk) * TQ * (D + 2);
+            if (it.slot >= 0) {
+                float* part = p.partials + ((int64_t)it.slot * kv_units + sub) * TQ * (D + 2);
                 float4* po = reinterpret_cast<float4*>(part + r * D + c0);
                 po[0] = make_float4(v[0], v[1], v[2], v[3]);
                 po[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -652,77 +850,112 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     }
 }
 
-// One block per (split tile, K/V head, query row): the pieces' sums, in piece
-// order within each warp and the four warps in order (the result repeats).
-template <int D>
+// The sums of split tiles and windows: per (split, head, query row) the pieces
+// in order, by one warp, or by a block's four warps (each every fourth piece,
+// then the four in order) where there are too few rows to fill the blocks'
+// warps.  Which of the two follows from counts, so the result repeats.
+template <int D, bool PAGED>
 __global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p) {
     constexpr int E = D / 32;  // channels per lane
+    constexpr int AHEAD = 8;   // pieces read at a time
     __shared__ float s_o[4][D], s_l[4];
-    const Kv4PlanHeader* plan = p.plan;
-    const int tq = plan->tile_rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const Kv4Split* splits =
-        reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(plan + 1) + (int64_t)plan->items_cap * sizeof(Kv4Item));
-    const int64_t units = (int64_t)plan->num_splits * p.kv_heads * tq;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tq = PAGED ? p.plan->tile_rows : 16, subs = PAGED ? p.kv_heads : p.heads;
+    const int count = PAGED ? p.plan->num_splits : min(p.pieces->splits, p.splits_cap);
+    const int live_rows = PAGED ? min(tq, max(p.group, 1)) : tq;  // of a tile of one token
+    const int64_t units = (int64_t)count * subs * tq;
+    const bool team = (int64_t)count * subs * live_rows <= 4ll * gridDim.x;
+    const int64_t stride = (int64_t)subs * tq * (D + 2);  // from piece to piece
+    const int64_t first = team ? blockIdx.x : (int64_t)blockIdx.x * 4 + warp, step = (int64_t)gridDim.x * (team ? 1 : 4);
+    for (int64_t u = first; u < units; u += step) {
         const int r = (int)(u % tq);
-        const int64_t rest = u / tq;
-        const int hk = (int)(rest % p.kv_heads);
-        const Kv4Split s = splits[rest / p.kv_heads];
-        const int row = s.row0 + r;
-        if (row >= s.rows) continue;
-        const int64_t stride = (int64_t)p.kv_heads * tq * (D + 2);
-        const float* part = p.partials + ((int64_t)s.slot * p.kv_heads + hk) * tq * (D + 2);
+        const int sub = (int)(u / tq % subs), split = (int)(u / tq / subs);
+        int slot, parts;
+        int64_t dst;  // row of O, or -1
+        if constexpr (PAGED) {
+            const Kv4Split* splits = reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(p.plan + 1) +
+                                                                       (int64_t)p.plan->items_cap * sizeof(Kv4Item));
+            const Kv4Split s = splits[split];
+            const int row = s.row0 + r, tok = row / p.group;
+            slot = s.slot;
+            parts = s.parts;
+            dst = row < s.rows ? ((int64_t)(s.q_token + tok) * p.heads + sub * p.group + row - tok * p.group) : -1;
+        } else {
+            const int4 s = p.window_splits[split];
+            const int64_t row = (int64_t)(s.x - p.q_window_base) * 16 + r;
+            slot = s.y;
+            parts = s.z;
+            dst = s.x >= 0 && row < p.q_rows && (int64_t)s.x * 16 + r < p.num_nodes ? row * p.heads + sub : -1;
+        }
+        if (dst < 0) continue;  // for the whole team
+        const float* part = p.partials + (int64_t)slot * stride + (int64_t)sub * tq * (D + 2);
         const float2* ml = reinterpret_cast<const float2*>(part + tq * D + 2 * r);
+        const float* src = part + r * D + lane * E;
         float top = kNoReference;
-        for (int k = lane; k < s.parts; k += 32) top = fmaxf(top, ml[k * (stride / 2)].x);
+        for (int k = lane; k < parts; k += 32) top = fmaxf(top, ml[k * (stride / 2)].x);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         float v[E], l = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) v[i] = 0.f;
-        const float* src = part + r * D + lane * E;
-#pragma unroll 8
-        for (int k = warp; k < s.parts; k += 4) {
-            const float2 m = ml[k * (stride / 2)];
-            const float c = exp2_approx(m.x - top);
-            l = fmaf(c, m.y, l);
-            if constexpr (E == 4) {
-                const float4 x = *reinterpret_cast<const float4*>(src + k * stride);
-                v[0] = fmaf(c, x.x, v[0]);
-                v[1] = fmaf(c, x.y, v[1]);
-                v[2] = fmaf(c, x.z, v[2]);
-                v[3] = fmaf(c, x.w, v[3]);
-            } else {
-                const float2 x = *reinterpret_cast<const float2*>(src + k * stride);
-                v[0] = fmaf(c, x.x, v[0]);
-                v[1] = fmaf(c, x.y, v[1]);
+        const int k0 = team ? warp : 0, dk = team ? 4 : 1;
+        for (int k = k0; k < parts; k += dk * AHEAD) {
+            float2 m[AHEAD];
+            float x[AHEAD][E];
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                const int64_t at = (int64_t)min(k + a * dk, parts - 1) * stride;
+                m[a] = ml[at / 2];
+                if constexpr (E == 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(src + at);
+                    x[a][0] = y.x;
+                    x[a][1] = y.y;
+                    x[a][2] = y.z;
+                    x[a][3] = y.w;
+                } else {
+                    const float2 y = *reinterpret_cast<const float2*>(src + at);
+                    x[a][0] = y.x;
+                    x[a][1] = y.y;
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < AHEAD; ++a) {
+                if (k + a * dk < parts) {
+                    const float c = exp2_approx(m[a].x - top);
+                    l = fmaf(c, m[a].y, l);
+#pragma unroll
+                    for (int i = 0; i < E; ++i) v[i] = fmaf(c, x[a][i], v[i]);
+                }
             }
         }
+        if (team) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = v[i];
-        if (lane == 0) s_l[warp] = l;
-        __syncthreads();
-        if (threadIdx.x < D / 8) {
-            float den = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < E; ++i) s_o[warp][lane * E + i] = v[i];
+            if (lane == 0) s_l[warp] = l;
+            __syncthreads();
+            if (warp == 0) {
+                l = 0.f;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                den += s_l[w];
+                for (int i = 0; i < E; ++i) v[i] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) o[k] += s_o[w][threadIdx.x * 8 + k];
+                for (int w = 0; w < 4; ++w) {
+                    l += s_l[w];
+#pragma unroll
+                    for (int i = 0; i < E; ++i) v[i] += s_o[w][lane * E + i];
+                }
             }
-            const float inv = den != 0.f ? __frcp_rn(den) : 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) o[k] *= inv;
-            const int tok = row / p.group;
-            store_channels<8>(p.o, ((int64_t)(s.q_token + tok) * p.heads + hk * p.group + row - tok * p.group) * D + threadIdx.x * 8,
-                              o, p.o_dtype);
+            __syncthreads();
+            if (warp != 0) continue;
         }
-        __syncthreads();
+        const float inv = l != 0.f ? __frcp_rn(l) : 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) v[i] *= inv;
+        store_few<E>(p.o, dst * D + lane * E, v, p.o_dtype);
     }
 }
 
 template <int D, int NT, bool PAGED, bool PRECISE>
-static int attend_variant(const AttendParams& p, int64_t units, cudaStream_t stream) {
+static int attend_variant(const AttendParams& p, int64_t units, cudaStream_t stream) {  // units: an upper bound
     using C = AttendCfg<D, NT>;
     static PerContext<int> attr;
     const int rc = attr.get(nullptr, [](int* v) -> int {
@@ -732,8 +965,8 @@ static int attend_variant(const AttendParams& p, int64_t units, cudaStream_t str
         return F3S_SUCCESS;
     });
     if (rc != F3S_SUCCESS) return rc;
-    const int per_cta = PAGED ? 1 : kAttendWarps / p.warps_per_unit;
-    const int64_t grid = std::min<int64_t>((units + per_cta - 1) / per_cta, INT32_MAX);
+    // a CTA per item of a plan; by ticket, as many as run at the same time
+    const int64_t grid = std::min<int64_t>(units, PAGED ? INT32_MAX : C::MIN_CTAS * num_sms_of_current_device());
     if (grid == 0) return F3S_SUCCESS;
     k_attend4<D, NT, PAGED, PRECISE><<<(unsigned)grid, kAttendWarps * 32, C::SMEM, stream>>>(p);
     F3S_LAUNCH_CHECK();
@@ -768,7 +1001,7 @@ static int check_attend(const void* Q, int q_dtype, int64_t qt, int64_t qh, cons
 
 extern "C" {
 
-size_t f3s_kv4_attention_workspace_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
+size_t f3s_kv4_attention_scratch_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
                                         int32_t head_dim) {
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || num_requests < 0 || num_tokens < 0) return 0;
     if (head_dim != 64 && head_dim != 128) return 0;
@@ -780,8 +1013,8 @@ size_t f3s_kv4_attention_workspace_size(int32_t num_requests, int64_t num_tokens
 int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, int64_t q_head_stride,
                       const void* d_pages, int32_t num_pages, const int32_t* d_tables, int64_t table_stride,
                       void* d_plan, int32_t num_requests, int64_t num_tokens, int32_t heads,
-                      int32_t kv_heads, int32_t head_dim, float scale, void* d_O, int32_t o_dtype, void* d_workspace,
-                      size_t workspace_bytes, f3s_stream_t stream) {
+                      int32_t kv_heads, int32_t head_dim, float scale, void* d_O, int32_t o_dtype, void* d_scratch,
+                      size_t scratch_bytes, f3s_stream_t stream) {
     f3s::NvtxRange nvtx_("f3s_kv4_attention");
     if (num_requests < 0 || num_tokens < 0) return F3S_ERR_INVALID_VALUE;
     if (head_dim != 64 && head_dim != 128) return F3S_ERR_UNSUPPORTED;
@@ -791,11 +1024,11 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     if (rc != F3S_SUCCESS) return rc;
     if (num_tokens * (heads / kv_heads) > INT32_MAX / 4) return F3S_ERR_TOO_LARGE;
     if (!d_tables || !d_plan || (reinterpret_cast<uintptr_t>(d_plan) & 15)) return F3S_ERR_INVALID_VALUE;
-    if (!d_workspace || (reinterpret_cast<uintptr_t>(d_workspace) & 15)) return F3S_ERR_INVALID_VALUE;
+    if (!d_scratch || (reinterpret_cast<uintptr_t>(d_scratch) & 15)) return F3S_ERR_INVALID_VALUE;
     const f3s::Kv4PlanLayout L = f3s::kv4_plan_layout(num_requests, num_tokens, heads, kv_heads,
                                                       f3s::num_sms_of_current_device());
     if (L.items_cap > INT32_MAX / 4) return F3S_ERR_TOO_LARGE;
-    if (workspace_bytes < (size_t)L.slots_cap * kv_heads * L.tile_rows * (head_dim + 2) * 4) return F3S_ERR_WORKSPACE;
+    if (scratch_bytes < (size_t)L.slots_cap * kv_heads * L.tile_rows * (head_dim + 2) * 4) return F3S_ERR_WORKSPACE;
     f3s::AttendParams p{};
     p.q = d_Q;
     p.q_token = q_token_stride;
@@ -811,10 +1044,9 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     p.o_dtype = o_dtype;
     p.plan = static_cast<const f3s::Kv4PlanHeader*>(d_plan);
     p.status = &static_cast<f3s::WsHeader*>(d_plan)->status;
-    p.partials = static_cast<float*>(d_workspace);
+    p.partials = static_cast<float*>(d_scratch);
     p.tables = d_tables;
     p.table_stride = table_stride;
-    p.warps_per_unit = f3s::kAttendWarps;
     cudaStream_t s = (cudaStream_t)stream;
     const int64_t units = L.items_cap * kv_heads;
     int st;
@@ -824,20 +1056,27 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     if (st != F3S_SUCCESS) return st;
     const int64_t blocks = std::min<int64_t>((int64_t)L.splits_cap * kv_heads * L.tile_rows,
                                              8ll * f3s::num_sms_of_current_device());
-    if (head_dim == 64) f3s::k_attend4_merge<64><<<(unsigned)blocks, 128, 0, s>>>(p);
-    else f3s::k_attend4_merge<128><<<(unsigned)blocks, 128, 0, s>>>(p);
+    if (head_dim == 64) f3s::k_attend4_merge<64, true><<<(unsigned)blocks, 128, 0, s>>>(p);
+    else f3s::k_attend4_merge<128, true><<<(unsigned)blocks, 128, 0, s>>>(p);
     F3S_LAUNCH_CHECK();
     return F3S_SUCCESS;
 }
 
+size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t head_dim) {
+    if (num_items < 0 || num_blocks < 0 || heads <= 0 || (head_dim != 64 && head_dim != 128)) return 0;
+    return f3s::window_piece_layout(num_items, num_blocks, heads, head_dim, f3s::num_sms_of_current_device()).total;
+}
+
 int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32_t num_pages, void* d_O,
                     int32_t o_dtype, const int32_t* d_window_offsets, const int32_t* d_block_cols,
-                    const int32_t* d_order, int32_t num_items, int32_t num_nodes, int32_t heads, int32_t kv_heads,
-                    int32_t head_dim, float scale, int32_t q_window_base, int32_t q_rows, void* d_workspace,
-                    size_t workspace_bytes, f3s_stream_t stream) {
+                    const int32_t* d_order, int32_t num_items, int64_t num_blocks, int32_t num_nodes, int32_t heads,
+                    int32_t kv_heads, int32_t head_dim, float scale, int32_t q_window_base, int32_t q_rows,
+                    void* d_workspace, size_t workspace_bytes, void* d_scratch, size_t scratch_bytes,
+                    f3s_stream_t stream) {
     f3s::NvtxRange nvtx_("f3s_kv4_forward");
-    if (num_items < 0 || num_nodes < 0 || q_window_base < 0 || q_rows < 0) return F3S_ERR_INVALID_VALUE;
+    if (num_items < 0 || num_blocks < 0 || num_nodes < 0 || q_window_base < 0 || q_rows < 0) return F3S_ERR_INVALID_VALUE;
     if (head_dim != 64 && head_dim != 128) return F3S_ERR_UNSUPPORTED;
+    if (heads <= 0) return F3S_ERR_INVALID_VALUE;
     if (!d_workspace) return F3S_ERR_INVALID_VALUE;
     if (workspace_bytes < f3s::kWsHeaderBytes) return F3S_ERR_WORKSPACE;
     if (num_items == 0 || num_nodes == 0 || q_rows == 0) return F3S_SUCCESS;
@@ -847,6 +1086,8 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
     if (!d_window_offsets || !d_block_cols || !d_order) return F3S_ERR_INVALID_VALUE;
     const int windows = (int)(((int64_t)num_nodes + 15) / 16);
     if (num_pages < windows) return F3S_ERR_INVALID_VALUE;
+    if (!d_scratch || (reinterpret_cast<uintptr_t>(d_scratch) & 15)) return F3S_ERR_INVALID_VALUE;
+    if (scratch_bytes < f3s_kv4_forward_scratch_size(num_items, num_blocks, heads, head_dim)) return F3S_ERR_WORKSPACE;
     f3s::AttendParams p{};
     p.q = d_Q;
     p.q_token = (int64_t)heads * head_dim;
@@ -863,16 +1104,50 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
     p.status = &static_cast<f3s::WsHeader*>(d_workspace)->status;
     p.offsets = d_window_offsets;
     p.cols = d_block_cols;
-    p.order = d_order;
-    p.num_items = num_items;
     p.num_nodes = num_nodes;
     p.windows = windows;
     p.q_window_base = q_window_base;
     p.q_rows = q_rows;
-    const int64_t units = (int64_t)num_items * heads;
-    // one warp per window and head once that fills the SMs' warps
-    p.warps_per_unit = units >= 16ll * f3s::num_sms_of_current_device() ? 1 : f3s::kAttendWarps;
-    return f3s::attend_launch<2, false>(p, head_dim, units, (cudaStream_t)stream);
+    const int sms = f3s::num_sms_of_current_device();
+    const f3s::WindowPieceLayout L = f3s::window_piece_layout(num_items, num_blocks, heads, head_dim, sms);
+    const int64_t units = ((int64_t)num_items + L.heavy_cap) * heads;
+    if (units > INT32_MAX / 2) return F3S_ERR_TOO_LARGE;
+    char* base = static_cast<char*>(d_scratch);
+    f3s::WindowPieceParams w{};
+    w.offsets = d_window_offsets;
+    w.order = d_order;
+    w.num_items = num_items;
+    w.windows = windows;
+    w.q_window_base = q_window_base;
+    w.q_rows = q_rows;
+    w.light = L.light;
+    w.heavy = windows <= L.heavy ? INT32_MAX : L.heavy;  // no window has more blocks than there are columns
+    w.heavy_cap = (int)L.heavy_cap;
+    w.splits_cap = (int)L.splits_cap;
+    w.slots_cap = (int)L.slots_cap;
+    w.pieces = reinterpret_cast<f3s::WindowPieces*>(base);
+    w.heavy_items = reinterpret_cast<int4*>(base + L.heavy_items);
+    w.light_items = reinterpret_cast<int*>(base + L.light_items);
+    w.splits = reinterpret_cast<int4*>(base + L.splits);
+    w.status = p.status;
+    p.pieces = w.pieces;
+    p.heavy_items = w.heavy_items;
+    p.light_items = w.light_items;
+    p.window_splits = w.splits;
+    p.heavy_cap = w.heavy_cap;
+    p.splits_cap = w.splits_cap;
+    p.partials = reinterpret_cast<float*>(base + L.partials);
+    cudaStream_t s = (cudaStream_t)stream;
+    F3S_CUDA_TRY(cudaMemsetAsync(base, 0, sizeof(f3s::WindowPieces), s));
+    f3s::k_window_pieces<<<(unsigned)((num_items + 255) / 256), 256, 0, s>>>(w);
+    F3S_LAUNCH_CHECK();
+    const int st = f3s::attend_launch<2, false>(p, head_dim, units, s);
+    if (st != F3S_SUCCESS || L.splits_cap == 0 || w.heavy == INT32_MAX) return st;  // no window is split
+    const int64_t blocks = std::min<int64_t>(L.splits_cap * heads * 16, 8ll * sms);
+    if (head_dim == 64) f3s::k_attend4_merge<64, false><<<(unsigned)blocks, 128, 0, s>>>(p);
+    else f3s::k_attend4_merge<128, false><<<(unsigned)blocks, 128, 0, s>>>(p);
+    F3S_LAUNCH_CHECK();
+    return F3S_SUCCESS;
 }
 
 }  // extern "C"

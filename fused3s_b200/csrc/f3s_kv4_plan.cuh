@@ -62,7 +62,7 @@ inline Kv4PlanLayout kv4_plan_layout(int num_requests, int64_t num_tokens, int h
     L.tile_rows = mean <= 8 ? 8 : mean <= 16 ? 16 : 32;
     const int64_t tiles = rows / L.tile_rows + num_requests;
     // pieces for one wave: 4 (8 and 16 rows) or 2 (32) CTAs per SM
-    L.target = (int)std::max<int64_t>(1, (int64_t)sms * (L.tile_rows == 32 ? 2 : 4) / kv_heads);
+    L.target = (int)std::max<int64_t>(1, (int64_t)sms * (L.tile_rows == 32 ? 4 : 8) / kv_heads);
     L.items_cap = tiles + L.target;
     L.slots_cap = 2 * (int64_t)L.target;
     L.splits_cap = L.target;

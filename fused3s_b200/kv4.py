@@ -270,7 +270,7 @@ def attention_kv4(Q: torch.Tensor, cache: KV4Cache, bt: BlockTables, scale: floa
     if requests == 0 or bt.num_tokens == 0:
         return out
     with torch.cuda.device(device):
-        size = lib.f3s_kv4_attention_workspace_size(requests, bt.num_tokens, heads, cache.kv_heads, head_dim)
+        size = lib.f3s_kv4_attention_scratch_size(requests, bt.num_tokens, heads, cache.kv_heads, head_dim)
         ws = torch.empty(size, dtype=torch.uint8, device=device)
         st = lib.f3s_kv4_attention(q.data_ptr(), _IN_DTYPES[q.dtype], q.stride(0), q.stride(1), cache.pages.data_ptr(),
                                    cache.num_pages, bt.tables.data_ptr(), bt.tables.stride(0), bt.plan.data_ptr(),
@@ -324,10 +324,15 @@ def fused3s_forward_kv4(Q: torch.Tensor, cache: KV4Cache, fmt: BlockSparseFormat
     with torch.cuda.device(device):
         ws = _rows_workspace(device)
         stream = torch.cuda.current_stream(device).cuda_stream
+        items = order.shape[0]
+        blocks = fmt.num_blocks
+        size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, head_dim)
+        scratch = torch.empty(size, dtype=torch.uint8, device=device)
         st = lib.f3s_kv4_forward(q3.data_ptr(), _IN_DTYPES[Q.dtype], cache.pages.data_ptr(), cache.num_pages,
                                  out.data_ptr(), _OUT_DTYPES[out.dtype], fmt.window_offsets.data_ptr(), fmt.cols_ptr,
-                                 order.data_ptr(), order.shape[0], fmt.num_nodes, heads, cache.kv_heads, head_dim,
-                                 scale, q_window_base, q_rows, ws.data_ptr(), ws.numel(), stream)
+                                 order.data_ptr(), items, blocks, fmt.num_nodes, heads, cache.kv_heads, head_dim,
+                                 scale, q_window_base, q_rows, ws.data_ptr(), ws.numel(), scratch.data_ptr(), size,
+                                 stream)
         check(st, "f3s_kv4_forward")
         if check_status:
             check(lib.f3s_workspace_status(ws.data_ptr(), stream), "f3s_kv4_forward (device)")

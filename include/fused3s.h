@@ -492,20 +492,20 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
  *            the last new token are not written
  *   d_tables, table_stride, num_requests, num_tokens, heads, kv_heads: those that the plan was made with; d_plan is not changed but for
  *            its status, so several calls may share it
- *   d_workspace: f3s_kv4_attention_workspace_size bytes, 16-byte aligned, not
+ *   d_scratch: f3s_kv4_attention_scratch_size bytes, 16-byte aligned, not
  *            shared by calls that may overlap; needs no initialisation
  * A table entry of -1 holds no tokens (they are left out); one outside the
  * cache is too, and is reported as F3S_ERR_BAD_FORMAT in the plan's status.
  * fp16 and fp32 O are exact to fp32 arithmetic, bf16 O rounds the softmax
  * weights to fp16.
  * ---------------------------------------------------------------------- */
-size_t f3s_kv4_attention_workspace_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
+size_t f3s_kv4_attention_scratch_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
                                         int32_t head_dim);
 int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, int64_t q_head_stride,
                       const void* d_pages, int32_t num_pages, const int32_t* d_tables, int64_t table_stride,
                       void* d_plan, int32_t num_requests, int64_t num_tokens, int32_t heads,
-                      int32_t kv_heads, int32_t head_dim, float scale, void* d_O, int32_t o_dtype, void* d_workspace,
-                      size_t workspace_bytes, f3s_stream_t stream);
+                      int32_t kv_heads, int32_t head_dim, float scale, void* d_O, int32_t o_dtype, void* d_scratch,
+                      size_t scratch_bytes, f3s_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * f3s_forward over K / V held in 4 bits: block column c of the format is page
@@ -513,12 +513,19 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
  * are multiplied by `scale` (f3s_forward: 1); query head h reads K/V head
  * h / (heads / kv_heads); Q is contiguous fp16 or bf16.  Other arguments,
  * window lists and slabs as f3s_forward_ex.  num_pages >= ceil(num_nodes / 16).
+ * num_blocks (the active blocks of the listed windows, or an estimate) sets how
+ * heavy windows are cut into pieces for several SMs, merged in order, so no plan
+ * is needed; it does not change which blocks are computed.  d_workspace (f3s_forward_workspace_size bytes, zeroed once)
+ * keeps the status; d_scratch: f3s_kv4_forward_scratch_size bytes, 16-byte
+ * aligned, not shared by calls that may overlap, needs no initialisation.
  * ---------------------------------------------------------------------- */
+size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t head_dim);
 int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32_t num_pages, void* d_O,
                     int32_t o_dtype, const int32_t* d_window_offsets, const int32_t* d_block_cols,
-                    const int32_t* d_order, int32_t num_items, int32_t num_nodes, int32_t heads, int32_t kv_heads,
-                    int32_t head_dim, float scale, int32_t q_window_base, int32_t q_rows, void* d_workspace,
-                    size_t workspace_bytes, f3s_stream_t stream);
+                    const int32_t* d_order, int32_t num_items, int64_t num_blocks, int32_t num_nodes, int32_t heads,
+                    int32_t kv_heads, int32_t head_dim, float scale, int32_t q_window_base, int32_t q_rows,
+                    void* d_workspace, size_t workspace_bytes, void* d_scratch, size_t scratch_bytes,
+                    f3s_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -94,14 +94,15 @@ def test_c_calls_refuse_without_touching_the_gpu(lib):
     assert attend(n=0) == 0 and attend(r=0) == 0
 
     def forward(q=A, dt=1, pages=A, np_=4, o=A, off=A, cols=A, order=A, items=1, nodes=50, h=2, g=2, d=64, base=0,
-                rows=50, w=A, wb=256):
-        return lib.f3s_kv4_forward(q, dt, pages, np_, o, 0, off, cols, order, items, nodes, h, g, d, 1.0, base, rows,
-                                   w, wb, None)
+                rows=50, w=A, wb=256, s=A, sb=1 << 30, blocks=10):
+        return lib.f3s_kv4_forward(q, dt, pages, np_, o, 0, off, cols, order, items, blocks, nodes, h, g, d, 1.0, base,
+                                   rows, w, wb, s, sb, None)
 
     assert forward(q=None) == bad and forward(pages=None) == bad and forward(o=None) == bad
     assert forward(off=None) == bad and forward(cols=None) == bad and forward(order=None) == bad
     assert forward(np_=3) == bad and forward(h=3) == bad and forward(d=100) == unsupported
     assert forward(items=-1) == bad and forward(base=-1) == bad and forward(w=None) == bad and forward(wb=1) == ws
+    assert forward(s=None) == bad and forward(s=A + 4) == bad and forward(sb=100) == ws and forward(blocks=-1) == bad
     assert forward(items=0) == 0 and forward(nodes=0) == 0 and forward(rows=0) == 0
 
 
@@ -596,6 +597,12 @@ def test_graph_forward_many_units_empty_and_hub_windows(lib):
     assert (o[n // 2 + 16:] == 0).all()
     for _ in range(5):
         assert torch.equal(F.fused3s_forward_kv4(q, cache, fmt, scale=0.125), o)
+    # the hub alone, and listed more often than the format has blocks for
+    for order in ([4], [4] * 300):
+        out = torch.zeros_like(o)
+        F.fused3s_forward_kv4(q, cache, fmt, order=i32(order), out=out, scale=0.125, check_status=True)
+        R.assert_close(out[64:80], want[64:80], R.tolerance(q.double().cpu(), seen[0], seen[1], 0.125, want[64:80], torch.float32))
+        assert not out[:64].any() and not out[80:].any()
 
 
 @gpu
