@@ -396,12 +396,16 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         const int own = steps ? (steps - 1) * PP + min(PP, mine - (steps - 1) * PP * wpu) : 0;
         const int limit_id = PAGED ? p.num_pages : p.windows;
 
-        // ---- page ids, 32 at a time (one per lane), the next 32 ahead
+        // ---- page ids, 32 at a time (one per lane), the next 32 ahead; `flags`
+        // marks those that need a look before their scores count: no page, or
+        // the graph's last block column
+        const int* mine_at = list + first + wq * PP;
+        auto id_at = [&](int i) { return __ldg(mine_at + (int64_t)(i / PP) * PP * wpu + i % PP); };
         auto load_ids = [&](int batch) {
             const int i = batch * 32 + lane;
-            int id = 0;
+            int id = -1;
             if (i < own) {
-                id = __ldg(list + first + wq * PP + (int64_t)(i / PP) * PP * wpu + i % PP);
+                id = id_at(i);
                 if (id < 0 || id >= limit_id) {
                     if (!(PAGED && id == -1)) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
                     id = -1;
@@ -409,22 +413,24 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             }
             return id;
         };
+        auto flags_of = [&](int id) {
+            return __ballot_sync(0xffffffffu, id < 0 || (!PAGED && id == p.windows - 1));
+        };
         int ids = load_ids(0), ids_next = 0;
-        uint32_t skip = 0, tail = 0;  // of the pages in flight, bit (page index % 32)
+        uint32_t flags = flags_of(ids), flags_now = 0;  // of the batch last issued, of the one at work
+        const uint8_t* head_pages = p.pages + (int64_t)hk * RB;
         auto issue = [&](int step) {
             const int i = step * PP;
             if ((i & 31) == 0) {
-                if (i > 0) ids = ids_next;
+                if (i > 0) {
+                    ids = ids_next;
+                    flags = flags_of(ids);
+                }
                 if (i + 32 < own) ids_next = load_ids(i / 32 + 1);
             }
             int id[PP];
 #pragma unroll
-            for (int k = 0; k < PP; ++k) {
-                id[k] = __shfl_sync(0xffffffffu, ids, (i + k) & 31);
-                const uint32_t bit = 1u << ((i + k) & 31);
-                skip = id[k] < 0 || i + k >= own ? skip | bit : skip & ~bit;
-                if constexpr (!PAGED) tail = id[k] == p.windows - 1 ? tail | bit : tail & ~bit;
-            }
+            for (int k = 0; k < PP; ++k) id[k] = __shfl_sync(0xffffffffu, ids, (i + k) & 31);
             const uint32_t n = used + step, st = n % STAGES;
             if (lane == 0) {
                 const int have = min(PP, own - i);
@@ -432,8 +438,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 #pragma unroll
                 for (int k = 0; k < PP; ++k)
                     if (k < have)
-                        bulk_load(ring_a + st * C::STAGE_BYTES + k * RB,
-                                  p.pages + (int64_t)max(id[k], 0) * page_bytes + (int64_t)hk * RB, RB, bars + 8 * st);
+                        bulk_load(ring_a + st * C::STAGE_BYTES + k * RB, head_pages + (int64_t)max(id[k], 0) * page_bytes,
+                                  RB, bars + 8 * st);
             }
         };
         for (int i = 0; i < min(steps, STAGES); ++i) issue(i);
@@ -622,17 +628,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                     }
             }
             // ---- masks: only where a page has tokens that some row must not see
-            const int page = i * PP;  // of this warp's pages
             const int tok0 = PAGED ? (it.page0 + wq * PP + i * PP * wpu) * 16 : 0;
-            const uint32_t pages_bits = (PP == 2 ? 3u : 1u) << (page & 31);
-            bool masked;
-            if constexpr (PAGED) masked = (skip & pages_bits) || tok0 + 16 * PP > open;
-            else masked = (skip | tail) & pages_bits;
-            if (masked) {
+            if ((i * PP & 31) == 0) flags_now = flags;  // no later batch has been issued yet
+            if ((PAGED && tok0 + 16 * PP > open) || (flags_now >> (i * PP & 31) & (PP == 2 ? 3u : 1u))) {
+                __syncwarp();
 #pragma unroll
                 for (int k = 0; k < PP; ++k) {
-                    const bool skipped = (skip >> ((page + k) & 31)) & 1;
-                    const bool last = (tail >> ((page + k) & 31)) & 1;
+                    const int id = i * PP + k < own ? id_at(i * PP + k) : -1;
+                    const bool skipped = id < 0 || id >= limit_id;
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -644,21 +647,30 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                                 const int row = min(it.row0 + nt * 8 + 2 * t + (c & 1), it.rows - 1);
                                 hide = tok0 + 16 * k + tk > it.context + row / p.group;
                             } else {
-                                hide = last && (p.windows - 1) * 16 + tk >= p.num_nodes;
+                                hide = id == p.windows - 1 && id * 16 + tk >= p.num_nodes;
                             }
                             if (hide || skipped) x[k][nt][c] = -INFINITY;
                         }
+                    // a hidden token's scale and zero may be anything: its weight of 0
+                    // must stay 0 (where it is seen, a NaN is in the weight already)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        if (!(fabsf(ri[k][c]) < INFINITY)) ri[k][c] = 0.f;
+                        if (!(fabsf(vz[k][c]) < INFINITY)) vz[k][c] = 0.f;
+                    }
                 }
             }
             // ---- weights
-            float most = -INFINITY;
+            bool over = false;
 #pragma unroll
-            for (int k = 0; k < PP; ++k)
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int j = 0; j < 2; ++j) {
+                    const float most = ref[nt][j] + kRescaleAt;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) most = fmaxf(most, x[k][nt][c] - ref[nt][c & 1]);
-            if (__any_sync(0xffffffffu, most > kRescaleAt)) {
+                    for (int k = 0; k < PP; ++k) over = over || x[k][nt][j] > most || x[k][nt][j + 2] > most;
+                }
+            if (__any_sync(0xffffffffu, over)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -689,34 +701,18 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 #pragma unroll
                     for (int c = 0; c < 4; ++c) a[c] = exp2_approx(x[k][nt][c] - ref[nt][c & 1]);
                     const uint32_t h0 = pack_half2(a[0], a[1]), h1 = pack_half2(a[2], a[3]);
-                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                    const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
                     pb[nt][0] = movmatrix_t(h0);
                     pb[nt][1] = movmatrix_t(h1);
                     if constexpr (PRECISE) {
+                        const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
+                        const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
                         pl[nt][0] = movmatrix_t(pack_half2(a[0] - r0.x, a[1] - r0.y));
                         pl[nt][1] = movmatrix_t(pack_half2(a[2] - r1.x, a[3] - r1.y));
-                    } else {
-                        // the sums take the weights that the product takes
-                        a[0] = r0.x;
-                        a[1] = r0.y;
-                        a[2] = r1.x;
-                        a[3] = r1.y;
                     }
-                    if (masked) {
-                        // a masked token's scale and zero may be anything, NaN too
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const bool on = x[k][nt][c] != -INFINITY;
-                            den[nt][c & 1] += on ? a[c] * ri[k][c / 2] : 0.f;
-                            off[nt][c & 1] += on ? a[c] * vz[k][c / 2] : 0.f;
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            den[nt][c & 1] = fmaf(a[c], ri[k][c / 2], den[nt][c & 1]);
-                            off[nt][c & 1] = fmaf(a[c], vz[k][c / 2], off[nt][c & 1]);
-                        }
+                    for (int c = 0; c < 4; ++c) {
+                        den[nt][c & 1] = fmaf(a[c], ri[k][c / 2], den[nt][c & 1]);
+                        off[nt][c & 1] = fmaf(a[c], vz[k][c / 2], off[nt][c & 1]);
                     }
                 }
                 // ---- O^T += V^T P^T
