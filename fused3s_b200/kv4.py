@@ -27,18 +27,31 @@ CUDA graph) and does not synchronise unless check_status is set.
 """
 from __future__ import annotations
 
-import dataclasses
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import check
-from .api import _OUT_DTYPES, _WS, BlockSparseFormat, _as_nhd, _default_device, generate_balanced_window_order
+from .api import _OUT_DTYPES, _WS, BlockSparseFormat, _default_device, generate_balanced_window_order
 
 PAGE_TOKENS = 16
 _RECORDS = {16 * d + 128: d for d in (64, 128)}
 _IN_DTYPES = {torch.float16: _lib.F3S_OUT_F16, torch.bfloat16: _lib.F3S_OUT_BF16}
+
+
+def _on(device: torch.device):
+    """The device to switch to for a call, or None where it is current already."""
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same number without the Stream object, where torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 class KV4Cache:
@@ -46,7 +59,7 @@ class KV4Cache:
     16 * head_dim + 128], contiguous, on a CUDA device.  Wraps the tensor; a
     page of zeros holds zeros."""
 
-    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim")
+    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim", "device")
 
     def __init__(self, pages: torch.Tensor):
         if pages.dtype != torch.uint8 or pages.dim() != 3:
@@ -54,7 +67,7 @@ class KV4Cache:
         self.num_pages, self.kv_heads, record = pages.shape
         if record not in _RECORDS:
             raise ValueError("a page record has 16 * head_dim + 128 bytes, head_dim 64 or 128")
-        if pages.device.type != "cuda":
+        if not pages.is_cuda:
             raise ValueError("pages must be on a CUDA device")
         if not pages.is_contiguous():
             raise ValueError("pages must be contiguous")
@@ -62,6 +75,7 @@ class KV4Cache:
             raise ValueError("a cache holds fewer than 2^27 pages")
         self.head_dim = _RECORDS[record]
         self.pages = pages
+        self.device = pages.device
 
 
 def empty_kv4_cache(num_pages: int, kv_heads: int, head_dim: int, device=None) -> KV4Cache:
@@ -81,23 +95,31 @@ def _check_i32(name: str, t: torch.Tensor, device: torch.device, dim: int = 1) -
         raise ValueError(f"{name} must be contiguous")
 
 
-def _check_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, device: torch.device) -> torch.Tensor:
-    """[rows, heads, head_dim] of fp16 or bf16 with any strides that keep
-    16-byte loads: head_dim contiguous, the others multiples of 8."""
+def _check_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, device: torch.device):
+    """(pointer, strides in elements) of [rows, heads, head_dim] fp16 or bf16 with any
+    strides that keep 16-byte loads: head_dim contiguous, the others multiples of 8."""
     if t.dtype not in _IN_DTYPES:
         raise TypeError(f"{name} must be float16 or bfloat16")
     if t.device != device:
         raise ValueError(f"{name} must be on {device}, with the cache")
-    t = _as_nhd(t)
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim:
+    shape, strides, ptr = t.shape, t.stride(), t.data_ptr()
+    if len(shape) == 2:
+        shape, strides = (shape[0], 1, shape[1]), (strides[0], 0, strides[1])
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim:
         raise ValueError(f"{name} must be [rows, {heads}, {head_dim}]")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    if strides[2] != 1 or (strides[0] | strides[1]) & 7 or ptr & 15:
         raise ValueError(f"{name}: head_dim must be contiguous and rows start on 16-byte boundaries")
-    return t
+    return ptr, strides
 
 
-def _rows_workspace(device: torch.device) -> torch.Tensor:
-    return _WS.get(device, "kv4", 256)
+_ROWS_WS = {}  # status words of store, load and the graph forward, one per device and stream
+
+
+def _rows_workspace(index: int, stream: int) -> torch.Tensor:
+    ws = _ROWS_WS.get((index, stream))
+    if ws is None:
+        ws = _ROWS_WS[(index, stream)] = _WS.get(torch.device("cuda", index), "kv4", 256)
+    return ws
 
 
 def store_kv4(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, cache: KV4Cache,
@@ -108,25 +130,28 @@ def store_kv4(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, cache: KV4C
     in fp16, a whole zero, codes rounded half to even (include/fused3s.h).
     Slots must differ.  check_status: synchronise and raise if a slot lies
     outside the cache (such rows are skipped)."""
-    device = cache.pages.device
+    device = cache.device
     _check_i32("slots", slots, device)
-    k = _check_rows("K", K, cache.kv_heads, cache.head_dim, device)
-    v = _check_rows("V", V, cache.kv_heads, cache.head_dim, device)
+    k, ks = _check_rows("K", K, cache.kv_heads, cache.head_dim, device)
+    v, vs = _check_rows("V", V, cache.kv_heads, cache.head_dim, device)
     n = slots.shape[0]
-    if k.dtype != v.dtype:
+    if K.dtype != V.dtype:
         raise TypeError("K and V must have the same type")
-    if k.shape[0] != n or v.shape[0] != n:
+    if K.shape[0] != n or V.shape[0] != n:
         raise ValueError("K, V and slots must have the same number of rows")
+    switch = _on(device)
+    if switch is not None:
+        with switch:
+            return store_kv4(K, V, slots, cache, check_status)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        ws = _rows_workspace(device)
-        stream = torch.cuda.current_stream(device).cuda_stream
-        st = lib.f3s_kv4_store(k.data_ptr(), v.data_ptr(), _IN_DTYPES[k.dtype], k.stride(0), k.stride(1), v.stride(0),
-                               v.stride(1), slots.data_ptr(), n, cache.pages.data_ptr(), cache.num_pages,
-                               cache.kv_heads, cache.head_dim, ws.data_ptr(), ws.numel(), stream)
+    stream = _raw_stream(device.index)
+    ws = _rows_workspace(device.index, stream).data_ptr()
+    st = lib.f3s_kv4_store(k, v, _IN_DTYPES[K.dtype], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), n,
+                           cache.pages.data_ptr(), cache.num_pages, cache.kv_heads, cache.head_dim, ws, 256, stream)
+    if st:
         check(st, "f3s_kv4_store")
-        if check_status:
-            check(lib.f3s_workspace_status(ws.data_ptr(), stream), "f3s_kv4_store (device)")
+    if check_status:
+        check(lib.f3s_workspace_status(ws, stream), "f3s_kv4_store (device)")
     return cache
 
 
@@ -134,46 +159,84 @@ def load_kv4(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
              check_status: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
     """K and V [n, kv_heads, head_dim] that the cache holds in slots[i] (int32;
     -1: zeros), rounded to `dtype` (float16, bfloat16 or float32)."""
-    device = cache.pages.device
+    device = cache.device
     _check_i32("slots", slots, device)
     if dtype not in _OUT_DTYPES:
         raise TypeError("dtype must be float32, float16 or bfloat16")
+    switch = _on(device)
+    if switch is not None:
+        with switch:
+            return load_kv4(cache, slots, dtype, check_status)
     n = slots.shape[0]
     k = torch.empty((n, cache.kv_heads, cache.head_dim), dtype=dtype, device=device)
     v = torch.empty_like(k)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        ws = _rows_workspace(device)
-        stream = torch.cuda.current_stream(device).cuda_stream
-        st = lib.f3s_kv4_load(cache.pages.data_ptr(), cache.num_pages, cache.kv_heads, cache.head_dim,
-                              slots.data_ptr(), n, k.data_ptr(), v.data_ptr(), _OUT_DTYPES[dtype], ws.data_ptr(),
-                              ws.numel(), stream)
+    stream = _raw_stream(device.index)
+    ws = _rows_workspace(device.index, stream).data_ptr()
+    st = lib.f3s_kv4_load(cache.pages.data_ptr(), cache.num_pages, cache.kv_heads, cache.head_dim, slots.data_ptr(), n,
+                          k.data_ptr(), v.data_ptr(), _OUT_DTYPES[dtype], ws, 256, stream)
+    if st:
         check(st, "f3s_kv4_load")
-        if check_status:
-            check(lib.f3s_workspace_status(ws.data_ptr(), stream), "f3s_kv4_load (device)")
+    if check_status:
+        check(lib.f3s_workspace_status(ws, stream), "f3s_kv4_load (device)")
     return k, v
 
 
-@dataclasses.dataclass
 class BlockTables:
-    """What build_block_tables made: the tables (the caller's tensor, with the
-    new pages appended), int32 per-token arrays and the attention plan."""
-    tables: torch.Tensor         # int32 [requests, width]
-    query_offsets: torch.Tensor  # int32 [requests + 1]: first new token of each request
-    positions: torch.Tensor      # int32 [num_tokens]: position of each new token in its request
-    slots: torch.Tensor          # int32 [num_tokens]: its slot in the cache, -1: none
-    free_begin: torch.Tensor     # int32 [1]: first page of the free list that is still free
-    plan: torch.Tensor           # device plan and status
-    num_tokens: int
-    heads: int
-    kv_heads: int
+    """What build_block_tables made.
+
+    tables         int32 [requests, width]: the caller's tensor, with the new pages appended
+    query_offsets  int32 [requests + 1]: first new token of each request
+    positions      int32 [num_tokens]: position of each new token in its request
+    slots          int32 [num_tokens]: its slot in the cache, -1: none
+    free_begin     int32 [1]: first page of the free list that is still free
+    num_tokens, heads, kv_heads: as passed; `buffer` holds the device plan, the
+    status and the arrays above."""
+
+    __slots__ = ("tables", "num_tokens", "heads", "kv_heads", "buffer", "plan_bytes", "requests", "_views")
+
+    def __init__(self, tables, num_tokens, heads, kv_heads, buffer, plan_bytes):
+        self.tables, self.num_tokens, self.heads, self.kv_heads = tables, num_tokens, heads, kv_heads
+        self.buffer, self.plan_bytes, self.requests, self._views = buffer, plan_bytes, tables.shape[0], None
+
+    def _array(self, k: int) -> torch.Tensor:
+        if self._views is None:
+            n = self.num_tokens
+            self._views = self.buffer.split_with_sizes((self.plan_bytes // 4, self.requests + 1, 1, n, n))
+        return self._views[k]
+
+    @property
+    def query_offsets(self) -> torch.Tensor:
+        return self._array(1)
+
+    @property
+    def free_begin(self) -> torch.Tensor:
+        return self._array(2)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._array(3)
+
+    @property
+    def slots(self) -> torch.Tensor:
+        return self._array(4)
 
     def status(self) -> int:
         """Synchronise and return (and clear) the status of the build and of
         the attentions run with it: F3S_SUCCESS, F3S_ERR_NO_PAGES, ..."""
-        with torch.cuda.device(self.plan.device):
-            return _lib.load().f3s_workspace_status(self.plan.data_ptr(),
-                                                    torch.cuda.current_stream(self.plan.device).cuda_stream)
+        device = self.buffer.device
+        with torch.cuda.device(device):
+            return _lib.load().f3s_workspace_status(self.buffer.data_ptr(), _raw_stream(device.index))
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan_bytes(index: int, requests: int, num_tokens: int, heads: int, kv_heads: int) -> int:
+    return _lib.load().f3s_block_tables_workspace_size(requests, num_tokens, heads, kv_heads)
+
+
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(index: int, requests: int, num_tokens: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    return _lib.load().f3s_kv4_attention_scratch_size(requests, num_tokens, heads, kv_heads, head_dim)
 
 
 def build_block_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, tables: torch.Tensor,
@@ -213,23 +276,26 @@ def build_block_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, table
         raise ValueError("heads must be a multiple of kv_heads")
     if num_tokens < 0:
         raise ValueError("num_tokens must not be negative")
+    switch = _on(device)
+    if switch is not None:
+        with switch:
+            return build_block_tables(context_lens, new_lens, tables, free_pages, free_begin, num_tokens, heads,
+                                      kv_heads, check_status)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        size = lib.f3s_block_tables_workspace_size(requests, num_tokens, heads, kv_heads)
-        if size == 0:
-            raise ValueError("too many tokens or heads for one call")
-        ints = size // 4
-        buf = torch.empty(ints + requests + 2 + 2 * num_tokens, dtype=torch.int32, device=device)
-        plan, offsets, begin, positions, slots = buf.split((ints, requests + 1, 1, num_tokens, num_tokens))
-        base = buf.data_ptr()
-        o = base + size
-        st = lib.f3s_block_tables(context_lens.data_ptr(), new_lens.data_ptr(), requests, tables.data_ptr(),
-                                  tables.stride(0), width, free_pages.data_ptr(), free_pages.shape[0],
-                                  None if free_begin is None else free_begin.data_ptr(), num_tokens, heads, kv_heads,
-                                  o, o + 4 * (requests + 2), o + 4 * (requests + 2 + num_tokens),
-                                  o + 4 * (requests + 1), base, size, torch.cuda.current_stream(device).cuda_stream)
+    size = _plan_bytes(device.index, requests, num_tokens, heads, kv_heads)
+    if size == 0:
+        raise ValueError("too many tokens or heads for one call")
+    buf = torch.empty(size // 4 + requests + 2 + 2 * num_tokens, dtype=torch.int32, device=device)
+    base = buf.data_ptr()
+    o = base + size
+    st = lib.f3s_block_tables(context_lens.data_ptr(), new_lens.data_ptr(), requests, tables.data_ptr(),
+                              tables.stride(0), width, free_pages.data_ptr(), free_pages.shape[0],
+                              None if free_begin is None else free_begin.data_ptr(), num_tokens, heads, kv_heads,
+                              o, o + 4 * (requests + 2), o + 4 * (requests + 2 + num_tokens), o + 4 * (requests + 1),
+                              base, size, _raw_stream(device.index))
+    if st:
         check(st, "f3s_block_tables")
-    bt = BlockTables(tables, offsets, positions, slots, begin, plan, num_tokens, heads, kv_heads)
+    bt = BlockTables(tables, num_tokens, heads, kv_heads, buf, size)
     if check_status:
         check(bt.status(), "f3s_block_tables (device)")
     return bt
@@ -250,36 +316,45 @@ def attention_kv4(Q: torch.Tensor, cache: KV4Cache, bt: BlockTables, scale: floa
     token are left as they were.  out_dtype: float32, float16 or bfloat16
     (default Q's).  check_status: synchronise and raise if a table entry lies
     outside the cache (such pages are left out)."""
-    device = cache.pages.device
-    heads, head_dim = bt.heads, cache.head_dim
-    if heads == 0 or bt.kv_heads != cache.kv_heads:
+    device = cache.device
+    heads, kv_heads, head_dim = bt.heads, cache.kv_heads, cache.head_dim
+    if heads == 0 or bt.kv_heads != kv_heads:
         raise ValueError("the block tables were built for other heads (pass heads and kv_heads to build_block_tables)")
-    q = _check_rows("Q", Q, heads, head_dim, device)
-    if q.shape[0] != bt.num_tokens:
+    q, qs = _check_rows("Q", Q, heads, head_dim, device)
+    if Q.shape[0] != bt.num_tokens:
         raise ValueError("Q must have num_tokens rows")
-    if bt.tables.device != device:
+    if bt.buffer.device != device:
         raise ValueError("the block tables and the cache must be on the same device")
-    if out is None:
-        out = torch.empty(Q.shape, dtype=out_dtype or Q.dtype, device=device)
-    elif out.shape != Q.shape or not out.is_contiguous() or out.device != device or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned tensor shaped like Q, with the cache")
-    if out.dtype not in _OUT_DTYPES:
-        raise ValueError("O must be float32, float16 or bfloat16")
-    requests = bt.tables.shape[0]
-    lib = _lib.load()
-    if requests == 0 or bt.num_tokens == 0:
+    out = _result(Q, out, out_dtype or Q.dtype, device)
+    if bt.requests == 0 or bt.num_tokens == 0:
         return out
-    with torch.cuda.device(device):
-        size = lib.f3s_kv4_attention_scratch_size(requests, bt.num_tokens, heads, cache.kv_heads, head_dim)
-        ws = torch.empty(size, dtype=torch.uint8, device=device)
-        st = lib.f3s_kv4_attention(q.data_ptr(), _IN_DTYPES[q.dtype], q.stride(0), q.stride(1), cache.pages.data_ptr(),
-                                   cache.num_pages, bt.tables.data_ptr(), bt.tables.stride(0), bt.plan.data_ptr(),
-                                   requests, bt.num_tokens, heads, cache.kv_heads, head_dim, scale, out.data_ptr(),
-                                   _OUT_DTYPES[out.dtype], ws.data_ptr(), size,
-                                   torch.cuda.current_stream(device).cuda_stream)
+    switch = _on(device)
+    if switch is not None:
+        with switch:
+            return attention_kv4(Q, cache, bt, scale, out, None, check_status)
+    lib = _lib.load()
+    size = _scratch_bytes(device.index, bt.requests, bt.num_tokens, heads, kv_heads, head_dim)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device)
+    st = lib.f3s_kv4_attention(q, _IN_DTYPES[Q.dtype], qs[0], qs[1], cache.pages.data_ptr(), cache.num_pages,
+                               bt.tables.data_ptr(), bt.tables.stride(0), bt.buffer.data_ptr(), bt.requests,
+                               bt.num_tokens, heads, kv_heads, head_dim, scale, out.data_ptr(), _OUT_DTYPES[out.dtype],
+                               scratch.data_ptr(), size, _raw_stream(device.index))
+    if st:
         check(st, "f3s_kv4_attention")
     if check_status:
         check(bt.status(), "f3s_kv4_attention (device)")
+    return out
+
+
+def _result(Q: torch.Tensor, out: Optional[torch.Tensor], dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if out is None:
+        if dtype not in _OUT_DTYPES:
+            raise ValueError("O must be float32, float16 or bfloat16")
+        return torch.empty(Q.shape, dtype=dtype, device=device)
+    if out.shape != Q.shape or not out.is_contiguous() or out.device != device or out.data_ptr() & 15:
+        raise ValueError("out must be a contiguous, 16-byte aligned tensor shaped like Q, with the cache")
+    if out.dtype not in _OUT_DTYPES:
+        raise ValueError("O must be float32, float16 or bfloat16")
     return out
 
 
@@ -296,44 +371,41 @@ def fused3s_forward_kv4(Q: torch.Tensor, cache: KV4Cache, fmt: BlockSparseFormat
     may be a multiple of its kv_heads (query head h reads K/V head
     h // (heads // kv_heads)).  order, out, q_window_base, check_status and
     out_dtype as in fused3s_forward."""
-    device = cache.pages.device
-    q3 = _as_nhd(Q)
-    if q3.dim() != 3 or q3.shape[2] != cache.head_dim or q3.shape[1] == 0 or q3.shape[1] % cache.kv_heads:
+    device = cache.device
+    q_rows, heads, head_dim = Q.shape if Q.dim() == 3 else (Q.shape[0], 1, Q.shape[-1])
+    if Q.dim() not in (2, 3) or head_dim != cache.head_dim or heads == 0 or heads % cache.kv_heads:
         raise ValueError("Q must be [rows, heads, head_dim] with the cache's head_dim and heads a multiple of its kv_heads")
-    q_rows, heads, head_dim = q3.shape
-    _check_rows("Q", Q, heads, head_dim, device)
+    q, _ = _check_rows("Q", Q, heads, head_dim, device)
     if not Q.is_contiguous():
         raise ValueError("Q must be contiguous")
     if fmt.window_offsets.device != device:
         raise ValueError("the format and the cache must be on the same device")
     if cache.num_pages < fmt.num_row_windows:
         raise ValueError("the cache must have a page for every block column of the graph")
+    switch = _on(device)
+    if switch is not None:
+        with switch:
+            return fused3s_forward_kv4(Q, cache, fmt, order, out, q_window_base, check_status, scale, out_dtype)
     if order is None:
         if q_window_base == 0 and q_rows == fmt.num_nodes:
             order = generate_balanced_window_order(fmt)
         else:
             order = torch.arange(q_window_base, q_window_base + (q_rows + 15) // 16, dtype=torch.int32, device=device)
-    order = order.to(device=device, dtype=torch.int32).contiguous()
-    if out is None:
-        out = torch.empty(Q.shape, dtype=out_dtype, device=device)
-    elif out.shape != Q.shape or not out.is_contiguous() or out.device != device or out.data_ptr() % 16:
-        raise ValueError("out must be a contiguous, 16-byte aligned tensor shaped like Q, with the cache")
-    if out.dtype not in _OUT_DTYPES:
-        raise ValueError("O must be float32, float16 or bfloat16")
+    elif order.dtype != torch.int32 or order.device != device or not order.is_contiguous():
+        order = order.to(device=device, dtype=torch.int32).contiguous()
+    out = _result(Q, out, out_dtype, device)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        ws = _rows_workspace(device)
-        stream = torch.cuda.current_stream(device).cuda_stream
-        items = order.shape[0]
-        blocks = fmt.num_blocks
-        size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, head_dim)
-        scratch = torch.empty(size, dtype=torch.uint8, device=device)
-        st = lib.f3s_kv4_forward(q3.data_ptr(), _IN_DTYPES[Q.dtype], cache.pages.data_ptr(), cache.num_pages,
-                                 out.data_ptr(), _OUT_DTYPES[out.dtype], fmt.window_offsets.data_ptr(), fmt.cols_ptr,
-                                 order.data_ptr(), items, blocks, fmt.num_nodes, heads, cache.kv_heads, head_dim,
-                                 scale, q_window_base, q_rows, ws.data_ptr(), ws.numel(), scratch.data_ptr(), size,
-                                 stream)
+    stream = _raw_stream(device.index)
+    ws = _rows_workspace(device.index, stream).data_ptr()
+    items, blocks = order.numel(), fmt.num_blocks
+    size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, head_dim)
+    scratch = torch.empty(size, dtype=torch.uint8, device=device)
+    st = lib.f3s_kv4_forward(q, _IN_DTYPES[Q.dtype], cache.pages.data_ptr(), cache.num_pages, out.data_ptr(),
+                             _OUT_DTYPES[out.dtype], fmt.window_offsets.data_ptr(), fmt.cols_ptr, order.data_ptr(), items,
+                             blocks, fmt.num_nodes, heads, cache.kv_heads, head_dim, scale, q_window_base, q_rows, ws, 256,
+                             scratch.data_ptr(), size, stream)
+    if st:
         check(st, "f3s_kv4_forward")
-        if check_status:
-            check(lib.f3s_workspace_status(ws.data_ptr(), stream), "f3s_kv4_forward (device)")
+    if check_status:
+        check(lib.f3s_workspace_status(ws, stream), "f3s_kv4_forward (device)")
     return out
