@@ -85,7 +85,7 @@ SIGNATURES = {
     "f3s_kv4_attention_scratch_size": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
     "f3s_kv4_attention": (ctypes.c_int, [_P, _I32, _I64, _I64, _P, _I32, _P, _I64, _P, _I32, _I64, _I32, _I32,
                                          _I32, _F32, _P, _I32, _P, _SZ, _P]),
-    "f3s_kv4_forward_scratch_size": (_SZ, [_I32, _I64, _I32, _I32]),
+    "f3s_kv4_forward_scratch_size": (_SZ, [_I32, _I64, _I32, _I32, _I32]),
     "f3s_kv4_forward": (ctypes.c_int, [_P, _I32, _P, _I32, _P, _I32, _P, _P, _P, _I32, _I64, _I32, _I32, _I32, _I32,
                                        _F32, _I32, _I32, _P, _SZ, _P, _SZ, _P]),
     "f3s_probe_mma_sync": (ctypes.c_int, [_I32, _I32, ctypes.POINTER(ctypes.c_double), _P]),

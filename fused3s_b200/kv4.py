@@ -398,7 +398,7 @@ def fused3s_forward_kv4(Q: torch.Tensor, cache: KV4Cache, fmt: BlockSparseFormat
     stream = _raw_stream(device.index)
     ws = _rows_workspace(device.index, stream).data_ptr()
     items, blocks = order.numel(), fmt.num_blocks
-    size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, head_dim)
+    size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, cache.kv_heads, head_dim)
     scratch = torch.empty(size, dtype=torch.uint8, device=device)
     st = lib.f3s_kv4_forward(q, _IN_DTYPES[Q.dtype], cache.pages.data_ptr(), cache.num_pages, out.data_ptr(),
                              _OUT_DTYPES[out.dtype], fmt.window_offsets.data_ptr(), fmt.cols_ptr, order.data_ptr(), items,

@@ -519,7 +519,8 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
  * keeps the status; d_scratch: f3s_kv4_forward_scratch_size bytes, 16-byte
  * aligned, not shared by calls that may overlap, needs no initialisation.
  * ---------------------------------------------------------------------- */
-size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t head_dim);
+size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t kv_heads,
+                                    int32_t head_dim);
 int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32_t num_pages, void* d_O,
                     int32_t o_dtype, const int32_t* d_window_offsets, const int32_t* d_block_cols,
                     const int32_t* d_order, int32_t num_items, int64_t num_blocks, int32_t num_nodes, int32_t heads,
