@@ -113,6 +113,31 @@ struct NvtxRange {
     NvtxRange& operator=(const NvtxRange&) = delete;
 };
 
+// Programmatic dependent launch: a kernel launched with launch_after may begin
+// before the one before it in the stream has ended, once each block of that one
+// has called launch_dependents() or ended; it reads nothing of it before
+// wait_for_primary(), which every block calls (so that whatever follows this
+// kernel follows the one before it, too), and nothing that any kernel before
+// wrote with non-coherent loads.
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_primary() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+inline int launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream, A&&... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(block);
+    c.dynamicSmemBytes = smem;
+    c.stream = stream;
+    cudaLaunchAttribute a{};
+    a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    a.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &a;
+    c.numAttrs = 1;
+    F3S_CUDA_TRY(cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...));
+    return F3S_SUCCESS;
+}
+
 // The part of a plan one forward launch runs, and the K / V rows it holds:
 // pieces [begin, end) of the plan (end -1: to the last), K / V holding the
 // graph's rows 16 * kv_col_base ... 16 * kv_col_base + kv_rows - 1 (kv_rows -1:

@@ -78,12 +78,14 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         fence_mbar_init();
     }
     __syncwarp();
+    launch_dependents();
+    wait_for_primary();  // the plan
     const int item = blockIdx.x / p.kv_heads, hk = blockIdx.x - item * p.kv_heads;
     if (item >= p.plan->num_items) return;
     Kv4Item it;
     {
         const int4* src = reinterpret_cast<const int4*>(reinterpret_cast<const Kv4Item*>(p.plan + 1) + item);
-        const int4 a = __ldg(src), b = __ldg(src + 1);
+        const int4 a = src[0], b = src[1];
         it.request = a.x;
         it.q_token = a.y;
         it.row0 = a.z;
@@ -103,7 +105,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     // ---- page ids, 32 at a time (one per lane), the next 32 ahead; `flags`
     // marks entries without a page
     const int* mine_at = p.tables + (int64_t)it.request * p.table_stride + it.page0 + warp * PP;
-    auto id_at = [&](int i) { return __ldg(mine_at + (int64_t)(i / PP) * PP * kAttendWarps + i % PP); };
+    auto id_at = [&](int i) { return mine_at[(int64_t)(i / PP) * PP * kAttendWarps + i % PP]; };
     auto load_ids = [&](int batch) {
         const int i = batch * 32 + lane;
         int id = -1;
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + off + t * (D / 4));
 #pragma unroll
             for (int w = 0; w < W; ++w) {
-                raw[nt][w] = off >= 0 ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+                raw[nt][w] = off >= 0 ? src[w] : make_uint4(0, 0, 0, 0);
                 const uint32_t u[4] = {raw[nt][w].x, raw[nt][w].y, raw[nt][w].z, raw[nt][w].w};
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
@@ -503,6 +505,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 // The sums of split tiles: see merge_rows.
 template <int D>
 __global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p) {
+    wait_for_primary();  // the sums
     const Kv4PlanHeader* plan = p.plan;
     const int tq = plan->tile_rows, group = p.group;
     const Kv4Split* splits =
@@ -530,9 +533,7 @@ static int attend_variant(const AttendParams& p, int64_t units, cudaStream_t str
     if (rc != F3S_SUCCESS) return rc;
     if (units > INT32_MAX) return F3S_ERR_TOO_LARGE;
     if (units == 0) return F3S_SUCCESS;
-    k_attend4<D, NT, PRECISE><<<(unsigned)units, kAttendWarps * 32, C::SMEM, stream>>>(p);
-    F3S_LAUNCH_CHECK();
-    return F3S_SUCCESS;
+    return launch_after(k_attend4<D, NT, PRECISE>, (unsigned)units, kAttendWarps * 32, C::SMEM, stream, p);
 }
 
 template <int NT>
@@ -604,10 +605,7 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     if (st != F3S_SUCCESS) return st;
     const int64_t blocks = std::min<int64_t>((int64_t)L.splits_cap * kv_heads * L.tile_rows,
                                              8ll * f3s::num_sms_of_current_device());
-    if (head_dim == 64) f3s::k_attend4_merge<64><<<(unsigned)blocks, 128, 0, s>>>(p);
-    else f3s::k_attend4_merge<128><<<(unsigned)blocks, 128, 0, s>>>(p);
-    F3S_LAUNCH_CHECK();
-    return F3S_SUCCESS;
+    return f3s::launch_after(head_dim == 64 ? f3s::k_attend4_merge<64> : f3s::k_attend4_merge<128>, (unsigned)blocks, 128, 0, s, p);
 }
 
 }  // extern "C"

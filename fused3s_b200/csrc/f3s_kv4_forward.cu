@@ -24,7 +24,6 @@ namespace f3s {
 
 constexpr int kConsumers = 4;
 constexpr int kAttendThreads = (kConsumers + 1) * 32;
-constexpr int kRingHeadSteps = 16;  // stages times K/V heads per stage
 
 // The windows of a graph as work (k_window_pieces): item i is the i-th listed
 // window or its first piece, the other pieces of cut windows follow behind the
@@ -44,7 +43,7 @@ struct WindowParams {
     int kv_heads, heads, group;
     int hg;        // heads per unit, one per consumer warp (times 4 / hg warps)
     int kvs;       // K/V heads per stage
-    int stages;    // kRingHeadSteps / kvs
+    int stages;    // of the ring: RING_STEPS / kvs
     float scale;   // times log2(e)
     void* o;       // contiguous [rows, heads, D] of o_dtype
     int o_dtype;
@@ -58,8 +57,10 @@ struct WindowParams {
     int num_nodes, windows, q_window_base, q_rows;
 };
 
-// Pieces of at most `piece` blocks: a quarter of a block's even share of the
-// work (3 blocks per SM), and 16 per warp that takes them in any case.
+// Pieces of at most `piece` blocks: half of a thread block's even share of the
+// work (3 of them per SM; a quarter costs more in sums to add, all of it leaves a
+// tail: 470 + 9, 468 + 25 and 545 + 8 us for 40,009 nodes, d = 128), and 8 per warp
+// that takes them in any case.
 struct WindowPieceLayout {
     int piece;
     int64_t extra_cap, splits_cap, slots_cap;
@@ -75,9 +76,9 @@ static int window_head_group(int heads, int group) {
 static WindowPieceLayout window_piece_layout(int num_items, int64_t num_blocks, int heads, int group, int head_dim, int sms) {
     WindowPieceLayout L{};
     const int hg = window_head_group(heads, group);
-    const int64_t blocks = 4 * 3ll * sms;
+    const int64_t blocks = 2 * 3ll * sms;
     const int64_t share = (num_blocks * (heads / hg) + blocks - 1) / blocks;
-    L.piece = (int)std::min<int64_t>(std::max<int64_t>(share, 16 * (4 / hg)), 1 << 28);
+    L.piece = (int)std::min<int64_t>(std::max<int64_t>(share, 8 * (4 / hg)), 1 << 28);
     const int64_t cut = num_blocks / L.piece;
     L.extra_cap = cut;
     L.splits_cap = std::min<int64_t>(num_items, cut);
@@ -109,6 +110,7 @@ struct WindowPieceParams {
 // which its pieces are summed do not.
 __global__ void __launch_bounds__(256) k_window_pieces(const WindowPieceParams p) {
     __shared__ int s_scan[256 / 32 + 1], s_base[3];
+    launch_dependents();
     const int i = blockIdx.x * 256 + threadIdx.x;
     int window = 0, b0 = 0, nb = 0;
     bool live = i < p.num_items;
@@ -161,22 +163,22 @@ struct WindowCfg {
     static constexpr int RB = kv4_record_bytes(D);
     static constexpr int PP = 2;                // pages per step
     static constexpr int ACC = D / 8 * 4;       // accumulators per lane
-    static constexpr bool Q_SMEM = D > 64;
-    static constexpr int RING = kRingHeadSteps * PP * RB;
+    static constexpr int RING_STEPS = D == 64 ? 16 : 8;  // stages times K/V heads per stage
+    static constexpr int RING = RING_STEPS * PP * RB;
     static constexpr int TOKENS = RING;         // per warp: what the tokens of a step multiply by
     static constexpr int TOKEN_BYTES = 5 * 16 * 4 * PP;
     static constexpr int Q = TOKENS + kConsumers * TOKEN_BYTES;
-    static constexpr int Q_BYTES = Q_SMEM ? 16 * D * 2 : 0;  // per warp
+    static constexpr int Q_BYTES = 16 * D * 2;  // per warp
     static constexpr int BARS = Q + kConsumers * Q_BYTES;
-    static constexpr int NBARS = 2 * kRingHeadSteps + 4;
+    static constexpr int NBARS = 2 * RING_STEPS + 4;
     static constexpr int UNITS = BARS + NBARS * 8;      // two unit records
     static constexpr int FLAGS = UNITS + 2 * 32;        // per stage
-    static constexpr int SINK = FLAGS + kRingHeadSteps * 4;
+    static constexpr int SINK = FLAGS + RING_STEPS * 4;
     static constexpr int MERGE = (SINK + kConsumers * 4 + 127) / 128 * 128;  // two warps' sums, where warps share a head
     static constexpr int MERGE_WORDS = ACC + 8;         // per lane
     static constexpr int SMEM = MERGE;
     static constexpr int SMEM_SHARED = MERGE + 2 * 32 * MERGE_WORDS * 4;
-    static constexpr int MIN_CTAS = 3;
+    static constexpr int MIN_CTAS = D == 64 ? 4 : 3;
 };
 
 struct Unit {  // as the producer hands it to the consumers
@@ -230,7 +232,7 @@ __device__ __forceinline__ void window_produce(const WindowParams& p, uint32_t r
         auto load_ids = [&](int i0) {
             int id = -1;
             if (i0 + lane < count) {
-                id = __ldg(list + i0 + lane);
+                id = list[i0 + lane];
                 if (id < 0 || id >= p.windows) {
                     atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
                     id = -1;
@@ -280,8 +282,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
     constexpr int N = D / 8;     // products' column blocks: output channels t * D / 4 + c and + D / 8 + c, c < N
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t base = smem_addr(smem), full = base + C::BARS, empty = full + 8 * kRingHeadSteps;
-    const uint32_t unit_full = empty + 8 * kRingHeadSteps, unit_empty = unit_full + 16;
+    const uint32_t base = smem_addr(smem), full = base + C::BARS, empty = full + 8 * C::RING_STEPS;
+    const uint32_t unit_full = empty + 8 * C::RING_STEPS, unit_empty = unit_full + 16;
     Unit* unit_records = reinterpret_cast<Unit*>(smem + C::UNITS);
     int* stage_flags = reinterpret_cast<int*>(smem + C::FLAGS);
     const int hg = p.hg, turns = kConsumers / hg;  // warps that share a head take its steps in turn
@@ -298,6 +300,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
         fence_mbar_init();
     }
     __syncthreads();
+    launch_dependents();
+    wait_for_primary();  // the pieces
     if (warp == kConsumers) {
         const int groups = p.heads / hg;
         window_produce<D>(p, base, full, empty, unit_full, unit_empty, unit_records, stage_flags,
@@ -327,7 +331,6 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
         // ---- Q as fp16 times a power of two that brings the tile's largest to
         // [2^9, 2^10); channels whose codes come in units of 2^-24 another 2^4.
         // Lane (g, t): channels t * D / 4 ... of its rows
-        uint32_t qf[C::Q_SMEM ? 1 : W][8];  // rows g and g + 8: four words each
         uint64_t qs[2];  // sum of a row's q in the scores' unit, twice
         float unit_scale;
         {
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + row * p.q_token +
                                                                   (int64_t)head * p.q_head + t * (D / 4));
 #pragma unroll
-                for (int w = 0; w < W; ++w) raw[r][w] = row < p.q_rows ? __ldg(src + w) : make_uint4(0, 0, 0, 0);
+                for (int w = 0; w < W; ++w) raw[r][w] = row < p.q_rows ? src[w] : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int r = 0; r < 2; ++r)
@@ -359,10 +362,9 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 for (int i = 0; i < 2 * W * 4; ++i) {
                     const int r = i / (W * 4), w = i / 4 % W, n = i % 4;
                     const int64_t row = row0 + 8 * r;
-                    const uint32_t x = row < p.q_rows ? __ldg(reinterpret_cast<const uint32_t*>(
-                                                                  static_cast<const uint16_t*>(p.q) + row * p.q_token +
-                                                                  (int64_t)head * p.q_head + t * (D / 4)) + 4 * w + n)
-                                                      : 0;
+                    const uint32_t* at = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + row * p.q_token +
+                                                                           (int64_t)head * p.q_head + t * (D / 4));
+                    const uint32_t x = row < p.q_rows ? at[4 * w + n] : 0;
                     const float2 y = q_floats(x, p.q_bf16);
                     if (fabsf(y.x) < INFINITY) amax = fmaxf(amax, fabsf(y.x));
                     if (fabsf(y.y) < INFINITY) amax = fmaxf(amax, fabsf(y.y));
@@ -393,13 +395,9 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 if (w == 0) mma_16816_zero(sum, a0, 0x2c002c00u, 0x3c003c00u);
                 else mma_16816(sum, a0, 0x2c002c00u, 0x3c003c00u);
                 mma_16816(sum, a1, 0x2c002c00u, 0x3c003c00u);
-                if constexpr (C::Q_SMEM) {  // each lane reads back what it wrote itself
-                    qsm[2 * w * 32 + lane] = make_uint4(h[0], h[4], h[1], h[5]);
-                    qsm[(2 * w + 1) * 32 + lane] = make_uint4(h[2], h[6], h[3], h[7]);
-                } else {
-#pragma unroll
-                    for (int n = 0; n < 8; ++n) qf[w][n] = h[n];
-                }
+                // each lane reads back what it wrote itself
+                qsm[2 * w * 32 + lane] = make_uint4(h[0], h[4], h[1], h[5]);
+                qsm[(2 * w + 1) * 32 + lane] = make_uint4(h[2], h[6], h[3], h[7]);
             }
             const float s0 = sum[0] * 9.5367431640625e-7f, s1 = sum[2] * 9.5367431640625e-7f;  // 2^-20
             qs[0] = pair(s0, s0);
@@ -455,15 +453,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
 #pragma unroll
                 for (int w = 0; w < W; ++w) {
                     const uint32_t g8 = kg[w] >> 8, h8 = kh[w] >> 8;
-                    uint32_t a0[4], a1[4];
-                    if constexpr (C::Q_SMEM) {
-                        const uint4 a = qsm[2 * w * 32 + lane], b = qsm[(2 * w + 1) * 32 + lane];
-                        a0[0] = a.x, a0[1] = a.y, a0[2] = a.z, a0[3] = a.w;
-                        a1[0] = b.x, a1[1] = b.y, a1[2] = b.z, a1[3] = b.w;
-                    } else {
-                        a0[0] = qf[w][0], a0[1] = qf[w][4], a0[2] = qf[w][1], a0[3] = qf[w][5];
-                        a1[0] = qf[w][2], a1[1] = qf[w][6], a1[2] = qf[w][3], a1[3] = qf[w][7];
-                    }
+                    const uint4 a = qsm[2 * w * 32 + lane], b = qsm[(2 * w + 1) * 32 + lane];
+                    const uint32_t a0[4] = {a.x, a.y, a.z, a.w}, a1[4] = {b.x, b.y, b.z, b.w};
                     if (w == 0) {
                         mma_16816_zero(s[0], a0, kg[w] & kNib0, kg[w] & kNib1);
                         mma_16816_zero(s[1], a0, kh[w] & kNib0, kh[w] & kNib1);
@@ -683,6 +674,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
 // The sums of cut windows: see merge_rows.
 template <int D>
 __global__ void __launch_bounds__(128) k_window_merge(const WindowParams p) {
+    wait_for_primary();  // the sums
     merge_rows<D>(min(p.pieces->splits, p.splits_cap), p.heads, 16, 16, p.partials, p.o, p.o_dtype,
                   [&](int split, int head, int r, int& slot, int& parts) -> int64_t {
                       const int4 s = p.window_splits[split];
@@ -705,10 +697,8 @@ static int window_launch(const WindowParams& p, int64_t units, cudaStream_t stre
     });
     if (rc != F3S_SUCCESS) return rc;
     const int64_t grid = std::min<int64_t>(units, C::MIN_CTAS * num_sms_of_current_device());
-    k_window_attend4<D, PRECISE>
-        <<<(unsigned)grid, kAttendThreads, p.hg < kConsumers ? C::SMEM_SHARED : C::SMEM, stream>>>(p);
-    F3S_LAUNCH_CHECK();
-    return F3S_SUCCESS;
+    return launch_after(k_window_attend4<D, PRECISE>, (unsigned)grid, kAttendThreads,
+                        p.hg < kConsumers ? C::SMEM_SHARED : C::SMEM, stream, p);
 }
 
 }  // namespace f3s
@@ -765,7 +755,7 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
     p.q_rows = q_rows;
     p.hg = f3s::window_head_group(heads, p.group);
     p.kvs = p.hg > p.group ? p.hg / p.group : 1;
-    p.stages = f3s::kRingHeadSteps / p.kvs;
+    p.stages = (head_dim == 64 ? f3s::WindowCfg<64>::RING_STEPS : f3s::WindowCfg<128>::RING_STEPS) / p.kvs;
     const int sms = f3s::num_sms_of_current_device();
     const f3s::WindowPieceLayout L = f3s::window_piece_layout(num_items, num_blocks, heads, p.group, head_dim, sms);
     const int64_t units = ((int64_t)num_items + L.extra_cap) * (heads / p.hg);
@@ -804,10 +794,7 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
                                   : (precise ? f3s::window_launch<128, true>(p, units, s) : f3s::window_launch<128, false>(p, units, s));
     if (st != F3S_SUCCESS || L.splits_cap == 0 || w.piece == INT32_MAX) return st;  // no window is split
     const int64_t blocks = std::min<int64_t>(L.splits_cap * heads * 16, 8ll * sms);
-    if (head_dim == 64) f3s::k_window_merge<64><<<(unsigned)blocks, 128, 0, s>>>(p);
-    else f3s::k_window_merge<128><<<(unsigned)blocks, 128, 0, s>>>(p);
-    F3S_LAUNCH_CHECK();
-    return F3S_SUCCESS;
+    return f3s::launch_after(head_dim == 64 ? f3s::k_window_merge<64> : f3s::k_window_merge<128>, (unsigned)blocks, 128, 0, s, p);
 }
 
 }  // extern "C"
