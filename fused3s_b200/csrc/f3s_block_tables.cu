@@ -30,8 +30,8 @@ struct BlockTablesParams {
     int num_free;
     const int* begin;
     int64_t num_tokens;
-    int group;  // 0: no plan
-    int tile_rows, target;
+    int group, tile_rows;
+    int target;  // 0: no plan
     int items_cap, splits_cap, slots_cap;
     int* query_offsets;
     int* positions;
@@ -43,56 +43,71 @@ struct BlockTablesParams {
     Kv4Split* splits;
 };
 
+// Sums stop here: what lies past it does not fit any array (num_tokens and the
+// plan's arrays are shorter), and two of them still add up in 32 bits.
+constexpr uint32_t kBtMost = 1u << 30;
+__device__ __forceinline__ uint32_t bt_add(uint32_t a, uint32_t b) { return min(a + b, kBtMost); }
+
 struct BtRequest {
-    int context, count;      // cached tokens, new tokens that have room
-    int old_pages, pages;    // table entries filled before, and after
+    int context, count;    // cached tokens, new tokens that have room
+    int old_pages, pages;  // table entries filled before, and after
     int tiles;
     int error;
 };
 
-// What fits of request r, whose new tokens start at `first` among all.
-__device__ __forceinline__ BtRequest bt_request(const BlockTablesParams& p, int c, int n, int64_t first) {
+// What fits of a request whose new tokens start at `first` among all.
+__device__ __forceinline__ BtRequest bt_request(const BlockTablesParams& p, int c, int n, uint32_t first) {
     BtRequest q;
     q.error = c < 0 || n < 0 ? F3S_ERR_INVALID_VALUE : 0;
     c = max(c, 0);
     n = max(n, 0);
-    const int64_t room_rows = p.num_tokens - first, room_table = (int64_t)p.width * 16 - c;
-    int64_t fit = n;
-    if (fit > room_rows) fit = max(room_rows, (int64_t)0);
-    if (fit > room_table) fit = max(room_table, (int64_t)0);
+    const int room_rows = max((int)p.num_tokens - (int)first, 0), room_table = p.width * 16 - c;
+    const int fit = min(min(n, room_rows), max(room_table, 0));
     if (fit < n || room_table < 0) q.error = q.error ? q.error : F3S_ERR_TOO_LARGE;
-    q.context = (int)min((int64_t)c, (int64_t)p.width * 16);
-    q.count = (int)fit;
-    q.old_pages = (q.context + 15) / 16;
-    q.pages = (int)(((int64_t)q.context + fit + 15) / 16);
-    q.tiles = p.group ? (int)((fit * p.group + p.tile_rows - 1) / p.tile_rows) : 0;
+    q.context = min(c, p.width * 16);
+    q.count = fit;
+    q.old_pages = (q.context + 15) >> 4;
+    q.pages = (q.context + fit + 15) >> 4;
+    q.tiles = (fit * p.group + p.tile_rows - 1) / p.tile_rows;
     return q;
 }
 
-__device__ __forceinline__ int64_t bt_scan(int64_t v, int64_t& total, int64_t* scratch) {
+// Exclusive sums of N values per thread over the block; total receives the
+// block's.  Two barriers, whatever N is.
+template <int N>
+__device__ __forceinline__ void bt_scan(uint32_t (&v)[N], uint32_t (&total)[N], uint32_t (*scratch)[kBtThreads / 32]) {
     const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-    int64_t inc = v;
+    uint32_t inc[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t n = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += n;
-    }
-    if (lane == 31) scratch[wid] = inc;
-    __syncthreads();
-    int64_t base = 0;
-    total = 0;
+    for (int k = 0; k < N; ++k) {
+        inc[k] = v[k];
 #pragma unroll
-    for (int i = 0; i < kBtThreads / 32; ++i) {
-        const int64_t s = scratch[i];
-        if (i < wid) base += s;
-        total += s;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t n = __shfl_up_sync(0xffffffffu, inc[k], o);
+            if (lane >= o) inc[k] = bt_add(inc[k], n);
+        }
+        if (lane == 31) scratch[k][wid] = inc[k];
     }
     __syncthreads();
-    return base + inc - v;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        // the warps' totals, scanned by every warp for itself
+        uint32_t w = lane < kBtThreads / 32 ? scratch[k][lane] : 0;
+#pragma unroll
+        for (int o = 1; o < kBtThreads / 32; o <<= 1) {
+            const uint32_t n = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w = bt_add(w, n);
+        }
+        total[k] = __shfl_sync(0xffffffffu, w, kBtThreads / 32 - 1);
+        uint32_t before = __shfl_up_sync(0xffffffffu, w, 1);
+        if (lane == 0) before = 0;
+        v[k] = bt_add(__shfl_sync(0xffffffffu, before, wid), __shfl_up_sync(0xffffffffu, inc[k], 1) * (lane > 0));
+    }
+    __syncthreads();
 }
 
 // Index of the request (0 ... n - 1) whose range [s[i], s[i + 1]) holds x.
-__device__ __forceinline__ int bt_find(const int64_t* s, int n, int64_t x) {
+__device__ __forceinline__ int bt_find(const uint32_t* s, int n, uint32_t x) {
     int lo = 0, hi = n;  // s[lo] <= x < s[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -108,16 +123,29 @@ __device__ __forceinline__ void bt_error(const BlockTablesParams& p, int code) {
 }
 
 __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesParams p) {
-    __shared__ int64_t s_first[kBtThreads + 1];  // first new token of each request of the chunk
-    __shared__ int64_t s_page[kBtThreads + 1];   // first new page
-    __shared__ int64_t s_item[kBtThreads + 1];   // first work item
-    __shared__ int64_t s_split[kBtThreads + 1];  // first split tile
-    __shared__ int64_t s_slot[kBtThreads + 1];   // first piece of a split tile
+    __shared__ uint32_t s_first[kBtThreads + 1];  // first new token of each request of the chunk
+    __shared__ uint32_t s_page[kBtThreads + 1];   // first new page
+    __shared__ uint32_t s_item[kBtThreads + 1];   // first work item
+    __shared__ uint32_t s_split[kBtThreads + 1];  // first split tile
+    __shared__ uint32_t s_slot[kBtThreads + 1];   // first piece of a split tile
     __shared__ BtRequest s_req[kBtThreads];
-    __shared__ int64_t s_scratch[kBtThreads / 32];
+    __shared__ uint32_t s_scratch[3][kBtThreads / 32];
+    __shared__ unsigned long long s_work;
+    launch_dependents();
     const int tid = threadIdx.x;
-    const int64_t at = (int64_t)blockIdx.x * kBtThreads + tid, step = (int64_t)gridDim.x * kBtThreads;
     const int chunks = (p.requests + kBtThreads - 1) / kBtThreads;
+    // half of the threads write slots, a quarter table entries, a quarter work items
+    const int role = tid / (kBtThreads / 4), at4 = tid % (kBtThreads / 4);
+    const uint32_t token_at = blockIdx.x * (kBtThreads / 2) + tid % (kBtThreads / 2), token_step = gridDim.x * (kBtThreads / 2);
+    const uint32_t other_at = blockIdx.x * (kBtThreads / 4) + at4, other_step = gridDim.x * (kBtThreads / 4);
+    int c0 = 0, n0 = 0;  // this thread's request of the first chunk
+    if (tid < p.requests) {
+        c0 = p.context[tid];
+        n0 = p.fresh[tid];
+    }
+    const int begin = p.begin ? max(p.begin[0], 0) : 0;
+    const uint32_t avail = (uint32_t)max(p.num_free - begin, 0);
+    if (tid == 0) s_work = 0;
     if (blockIdx.x == 0 && tid == 0) {
         p.ws->status = 0;
         p.ws->abort = 0;
@@ -125,159 +153,168 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
     __syncthreads();
 
     // pages that all tiles see together, which sets the size of a piece
-    int64_t piece = kKv4MinPiecePages;
-    int c0 = 0, n0 = 0;  // this thread's request of the first chunk
-    if (tid < p.requests) {
-        c0 = p.context[tid];
-        n0 = p.fresh[tid];
-    }
-    const int64_t begin = p.begin ? max(p.begin[0], 0) : 0;
-    const int64_t avail = max((int64_t)p.num_free - begin, (int64_t)0);
-    if (p.group) {
-        int64_t work = 0, base = 0;
-        for (int chunk = 0; chunk < chunks; ++chunk) {
-            const int r = chunk * kBtThreads + tid;
-            int c = c0, n = n0;
-            if (chunk) {
-                c = r < p.requests ? p.context[r] : 0;
-                n = r < p.requests ? p.fresh[r] : 0;
-            }
-            int64_t total, sum;
-            const int64_t first = base + bt_scan(max(n, 0), total, s_scratch);
-            base += total;
-            const BtRequest q = bt_request(p, c, n, first);
-            bt_scan(r < p.requests ? (int64_t)q.tiles * q.pages : 0, sum, s_scratch);
-            work += sum;
+    uint32_t v1[1], total1[1];
+    uint32_t first_base = 0, first0 = 0, tokens0 = 0;
+    unsigned long long work = 0;
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        const int r = chunk * kBtThreads + tid;
+        const int c = chunk == 0 ? c0 : r < p.requests ? p.context[r] : 0;
+        const int n = chunk == 0 ? n0 : r < p.requests ? p.fresh[r] : 0;
+        v1[0] = min((uint32_t)max(n, 0), kBtMost);
+        bt_scan<1>(v1, total1, s_scratch);
+        if (chunk == 0) {
+            first0 = v1[0];
+            tokens0 = total1[0];
         }
-        piece = max((work + p.target - 1) / p.target, (int64_t)kKv4MinPiecePages);
+        if (p.target == 0) break;  // no plan: the first chunk's sums are all that is kept
+        if (r < p.requests) {
+            const BtRequest q = bt_request(p, c, n, bt_add(first_base, v1[0]));
+            work += (unsigned long long)q.tiles * q.pages;
+        }
+        first_base = bt_add(first_base, total1[0]);
+    }
+    int piece = kKv4MinPiecePages;
+    if (p.target) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+        if ((tid & 31) == 0 && work) atomicAdd(&s_work, work);
+        __syncthreads();
+        piece = (int)min(max((s_work + p.target - 1) / p.target, (unsigned long long)kKv4MinPiecePages), 1ull << 28);
     }
 
-    int64_t first_base = 0, page_base = 0, item_base = 0, split_base = 0, slot_base = 0;
+    first_base = 0;
+    uint32_t page_base = 0, item_base = 0, split_base = 0, slot_base = 0;
     for (int chunk = 0; chunk < chunks; ++chunk) {
         const int r0 = chunk * kBtThreads, r = r0 + tid, here = min(kBtThreads, p.requests - r0);
         int c = c0, n = n0;
+        uint32_t first = first0, tokens = tokens0;
         if (chunk) {
             c = r < p.requests ? p.context[r] : 0;
             n = r < p.requests ? p.fresh[r] : 0;
+            v1[0] = min((uint32_t)max(n, 0), kBtMost);
+            bt_scan<1>(v1, total1, s_scratch);
+            first = bt_add(first_base, v1[0]);
+            tokens = total1[0];
         }
-        int64_t tokens, pages, items, splits, slots;
-        const int64_t first = first_base + bt_scan(max(n, 0), tokens, s_scratch);
         BtRequest q = bt_request(p, c, n, first);
         if (r >= p.requests) q = BtRequest{};
-        const int parts = q.tiles ? (int)((q.pages + piece - 1) / piece) : 0;
-        const int64_t page = page_base + bt_scan(q.pages - q.old_pages, pages, s_scratch);
-        const int64_t item = item_base + bt_scan((int64_t)q.tiles * parts, items, s_scratch);
-        const int64_t split = split_base + bt_scan(parts > 1 ? q.tiles : 0, splits, s_scratch);
-        const int64_t slot0 = slot_base + bt_scan(parts > 1 ? (int64_t)q.tiles * parts : 0, slots, s_scratch);
+        const int parts = q.tiles ? (q.pages + piece - 1) / piece : 0;
+        // new pages, items, and tiles cut in several (their slots are parts times as many)
+        uint32_t v[3] = {(uint32_t)(q.pages - q.old_pages), min((uint32_t)q.tiles * (uint32_t)parts, kBtMost),
+                         parts > 1 ? (uint32_t)q.tiles : 0u};
+        uint32_t total[3];
+        bt_scan<3>(v, total, s_scratch);
+        v1[0] = parts > 1 ? min((uint32_t)q.tiles * (uint32_t)parts, kBtMost) : 0u;
+        total1[0] = 0;
+        if (total[2]) bt_scan<1>(v1, total1, s_scratch);  // for the whole block
         if (q.error) bt_error(p, q.error);
         if (tid < here) {
             s_first[tid] = first;
-            s_page[tid] = page;
-            s_item[tid] = item;
-            s_split[tid] = split;
-            s_slot[tid] = slot0;
+            s_page[tid] = bt_add(page_base, v[0]);
+            s_item[tid] = bt_add(item_base, v[1]);
+            s_split[tid] = bt_add(split_base, v[2]);
+            s_slot[tid] = bt_add(slot_base, v1[0]);
             s_req[tid] = q;
-            if (blockIdx.x == 0 && p.query_offsets) p.query_offsets[r] = (int)min(first, (int64_t)INT32_MAX);
+            if (blockIdx.x == 0) p.query_offsets[r] = (int)first;
         }
+        const uint32_t token_end = bt_add(first_base, tokens), page_end = bt_add(page_base, total[0]),
+                       item_end = bt_add(item_base, total[1]);
         if (tid == 0) {
-            s_first[here] = first_base + tokens;
-            s_page[here] = page_base + pages;
-            s_item[here] = item_base + items;
-            s_split[here] = split_base + splits;
-            s_slot[here] = slot_base + slots;
+            s_first[here] = token_end;
+            s_page[here] = page_end;
+            s_item[here] = item_end;
         }
         __syncthreads();
-        // slots and positions of the chunk's tokens
-        const int64_t token_end = min(first_base + tokens, p.num_tokens);
-        for (int64_t t = first_base + at; t < token_end; t += step) {
-            const int i = bt_find(s_first, here, t);
-            const BtRequest& w = s_req[i];
-            const int64_t pos = (int64_t)w.context + (t - s_first[i]);
-            int slot = -1;
-            if (t - s_first[i] < w.count) {
-                const int k = (int)(pos >> 4);
-                int id = -1;
-                if (k < w.old_pages) {
-                    id = p.tables[(int64_t)(r0 + i) * p.stride + k];
-                } else {
-                    const int64_t f = s_page[i] + (k - w.old_pages);
-                    if (f < avail) id = p.free_pages[begin + f];
+        if (role < 2) {  // slots and positions of the chunk's tokens
+            const uint32_t end = min(token_end, (uint32_t)p.num_tokens);
+            for (uint32_t t = first_base + token_at; t < end; t += token_step) {
+                const int i = bt_find(s_first, here, t);
+                const BtRequest& w = s_req[i];
+                const int k = (int)(t - s_first[i]);
+                const int64_t pos = (int64_t)w.context + k;
+                int slot = -1;
+                if (k < w.count) {
+                    const int page = (int)(pos >> 4);
+                    int id = -1;
+                    if (page < w.old_pages) {
+                        id = p.tables[(int64_t)(r0 + i) * p.stride + page];
+                    } else {
+                        const uint32_t f = s_page[i] + (page - w.old_pages);
+                        if (f < avail) id = p.free_pages[begin + f];
+                    }
+                    // an entry that no cache can hold stays out of range, for the
+                    // store to report
+                    slot = id < 0 ? id : id < INT32_MAX / 16 ? id * 16 + (int)(pos & 15) : INT32_MAX;
                 }
-                // an entry that no cache can hold stays out of range, for the
-                // store to report
-                slot = id < 0 ? id : id < INT32_MAX / 16 ? id * 16 + (int)(pos & 15) : INT32_MAX;
+                p.slots[t] = slot;
+                p.positions[t] = (int)min(pos, (int64_t)INT32_MAX);
             }
-            p.slots[t] = slot;
-            p.positions[t] = (int)min(pos, (int64_t)INT32_MAX);
-        }
-        // the new entries of the chunk's table rows
-        for (int64_t f = page_base + at; f < page_base + pages; f += step) {
-            const int i = bt_find(s_page, here, f);
-            const int k = s_req[i].old_pages + (int)(f - s_page[i]);
-            p.tables[(int64_t)(r0 + i) * p.stride + k] = f < avail ? p.free_pages[begin + f] : -1;
-        }
-        // work items and split tiles
-        for (int64_t it = item_base + at; it < item_base + items; it += step) {
-            if (it >= p.items_cap) break;
-            const int i = bt_find(s_item, here, it);
-            const BtRequest& w = s_req[i];
-            const int m = (int)((w.pages + piece - 1) / piece);
-            const int local = (int)(it - s_item[i]);
-            const int tile = local / m, part = local - tile * m;
-            const int row0 = tile * p.tile_rows, rows = w.count * p.group;
-            const int last = min(row0 + p.tile_rows, rows) - 1;  // the tile's last row sees the most
-            const int64_t seen = ((int64_t)w.context + last / p.group) / 16 + 1;
-            Kv4Item d;
-            d.request = r0 + i;
-            d.q_token = (int)s_first[i];
-            d.row0 = row0;
-            d.rows = rows;
-            d.context = w.context;
-            d.page0 = (int)(seen * part / m);
-            d.page1 = (int)(seen * (part + 1) / m);
-            const int64_t slot = s_slot[i] + local;
-            d.slot = m > 1 && slot < p.slots_cap ? (int)slot : -1;
-            p.items[it] = d;
-            if (part == 0 && m > 1) {
-                const int64_t sp = s_split[i] + tile;
-                if (sp < p.splits_cap) {
-                    Kv4Split s{};
-                    s.slot = (int)slot;
-                    s.parts = m;
-                    s.q_token = d.q_token;
-                    s.row0 = row0;
-                    s.rows = rows;
-                    p.splits[sp] = s;
+        } else if (role == 2) {  // the new entries of the chunk's table rows
+            for (uint32_t f = page_base + other_at; f < page_end; f += other_step) {
+                const int i = bt_find(s_page, here, f);
+                const int k = s_req[i].old_pages + (int)(f - s_page[i]);
+                p.tables[(int64_t)(r0 + i) * p.stride + k] = f < avail ? p.free_pages[begin + f] : -1;
+            }
+        } else {  // work items and split tiles
+            for (uint32_t it = item_base + other_at; it < min(item_end, (uint32_t)p.items_cap); it += other_step) {
+                const int i = bt_find(s_item, here, it);
+                const BtRequest& w = s_req[i];
+                const int m = (w.pages + piece - 1) / piece;
+                const int local = (int)(it - s_item[i]);
+                const int tile = local / m, part = local - tile * m;
+                const int row0 = tile * p.tile_rows, rows = w.count * p.group;
+                const int last = min(row0 + p.tile_rows, rows) - 1;  // the tile's last row sees the most
+                const int seen = (w.context + last / p.group) / 16 + 1;
+                Kv4Item d;
+                d.request = r0 + i;
+                d.q_token = (int)s_first[i];
+                d.row0 = row0;
+                d.rows = rows;
+                d.context = w.context;
+                d.page0 = m == 1 ? 0 : (int)((int64_t)seen * part / m);
+                d.page1 = m == 1 ? seen : (int)((int64_t)seen * (part + 1) / m);
+                const uint32_t slot = s_slot[i] + local;
+                d.slot = m > 1 && slot < (uint32_t)p.slots_cap ? (int)slot : -1;
+                p.items[it] = d;
+                if (part == 0 && m > 1) {
+                    const uint32_t sp = s_split[i] + tile;
+                    if (sp < (uint32_t)p.splits_cap) {
+                        Kv4Split s{};
+                        s.slot = (int)slot;
+                        s.parts = m;
+                        s.q_token = d.q_token;
+                        s.row0 = row0;
+                        s.rows = rows;
+                        p.splits[sp] = s;
+                    }
                 }
             }
         }
-        first_base += tokens;
-        page_base += pages;
-        item_base += items;
-        split_base += splits;
-        slot_base += slots;
-        __syncthreads();  // the chunk's arrays are read no more
+        first_base = token_end;
+        page_base = page_end;
+        item_base = item_end;
+        split_base = bt_add(split_base, total[2]);
+        slot_base = bt_add(slot_base, total1[0]);
+        if (chunk + 1 < chunks) __syncthreads();  // the chunk's arrays are read no more
     }
     // slots behind the last token
-    for (int64_t t = first_base + at; t < p.num_tokens; t += step) {
+    for (uint32_t t = first_base + blockIdx.x * kBtThreads + tid; t < (uint32_t)p.num_tokens; t += gridDim.x * kBtThreads) {
         p.slots[t] = -1;
         p.positions[t] = 0;
     }
     if (blockIdx.x == 0 && tid == 0) {
-        p.query_offsets[p.requests] = (int)min(first_base, (int64_t)INT32_MAX);
-        p.begin_out[0] = (int)(begin + min(page_base, avail));
-        if (first_base > p.num_tokens) bt_error(p, F3S_ERR_TOO_LARGE);
+        p.query_offsets[p.requests] = (int)first_base;
+        p.begin_out[0] = begin + (int)min(page_base, avail);
+        if (first_base > (uint32_t)p.num_tokens) bt_error(p, F3S_ERR_TOO_LARGE);
         if (page_base > avail) bt_error(p, F3S_ERR_NO_PAGES);
-        if (p.plan) {
-            p.plan->num_items = (int)min(item_base, (int64_t)p.items_cap);
-            p.plan->num_splits = (int)min(split_base, (int64_t)p.splits_cap);
-            p.plan->items_cap = p.items_cap;
-            p.plan->splits_cap = p.splits_cap;
-            p.plan->tile_rows = p.tile_rows;
-            p.plan->group = p.group;
-            p.plan->num_requests = p.requests;
-            p.plan->num_tokens = (int)p.num_tokens;
-        }
+        p.plan->num_items = (int)min(item_base, (uint32_t)p.items_cap);
+        p.plan->num_splits = (int)min(split_base, (uint32_t)p.splits_cap);
+        p.plan->items_cap = p.items_cap;
+        p.plan->splits_cap = p.splits_cap;
+        p.plan->tile_rows = p.tile_rows;
+        p.plan->group = p.group;
+        p.plan->num_requests = p.requests;
+        p.plan->num_tokens = (int)p.num_tokens;
     }
 }
 
@@ -337,6 +374,7 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
     char* base = static_cast<char*>(d_plan);
     p.ws = static_cast<f3s::WsHeader*>(d_plan);
     p.plan = static_cast<f3s::Kv4PlanHeader*>(d_plan);
+    p.group = p.tile_rows = 1;
     int64_t units = std::max<int64_t>(num_tokens, 1);
     if (heads > 0) {
         const f3s::Kv4PlanLayout L = f3s::kv4_plan_layout(num_requests, num_tokens, heads, kv_heads,
@@ -353,7 +391,7 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
         p.splits = reinterpret_cast<f3s::Kv4Split*>(base + L.splits);
         units = std::max(units, L.items_cap);
     }
-    // one block per 1024 tokens (two per thread), a block per SM at most
+    // one block per 1024 tokens or items, a block per SM at most
     const int64_t blocks = std::min<int64_t>((units + 1023) / 1024, f3s::num_sms_of_current_device());
     f3s::k_block_tables<<<(unsigned)blocks, f3s::kBtThreads, 0, (cudaStream_t)stream>>>(p);
     F3S_LAUNCH_CHECK();
