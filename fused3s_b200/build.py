@@ -22,7 +22,7 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB = PKG / "libfused3s.so"
 SOURCES = ["f3s_api.cu", "f3s_block_tables.cu", "f3s_format.cu", "f3s_forward.cu", "f3s_kv4_attend.cu",
-           "f3s_kv4_forward.cu", "f3s_kv4_store.cu", "f3s_peer.cu", "f3s_probe.cu", "f3s_text.cu"]
+           "f3s_kv4_forward.cu", "f3s_kv4_prefill.cu", "f3s_kv4_store.cu", "f3s_peer.cu", "f3s_probe.cu", "f3s_text.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -15,29 +15,11 @@
 // rows share a page.
 //
 #include <algorithm>
-#include "f3s_kv4_math.cuh"
-#include "f3s_kv4_plan.cuh"
+#include "f3s_kv4_attend.cuh"
 
 namespace f3s {
 
 constexpr int kAttendWarps = 4;
-
-struct AttendParams {
-    const void* q;
-    int64_t q_token, q_head;  // strides in elements
-    int q_bf16;
-    const uint8_t* pages;
-    int num_pages;
-    int kv_heads, heads, group;
-    float scale;   // times log2(e)
-    void* o;       // contiguous [rows, heads, D] of o_dtype
-    int o_dtype;
-    int* status;
-    float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head
-    const Kv4PlanHeader* plan;
-    const int* tables;
-    int64_t table_stride;
-};
 
 template <int D, int NT>
 struct AttendCfg {
@@ -601,7 +583,8 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     int st;
     if (L.tile_rows == 8) st = f3s::attend_launch<1>(p, head_dim, units, s);
     else if (L.tile_rows == 16) st = f3s::attend_launch<2>(p, head_dim, units, s);
-    else st = f3s::attend_launch<4>(p, head_dim, units, s);
+    else if (L.tile_rows == 32) st = f3s::attend_launch<4>(p, head_dim, units, s);
+    else st = f3s::attend_tiles128(p, head_dim, units, s);
     if (st != F3S_SUCCESS) return st;
     const int64_t blocks = std::min<int64_t>((int64_t)L.splits_cap * kv_heads * L.tile_rows,
                                              8ll * f3s::num_sms_of_current_device());

@@ -7,7 +7,7 @@
 namespace f3s {
 
 // Query rows of one request and one K/V head are numbered row = token * group
-// + head within the group; a tile is tile_rows of them (8, 16 or 32), a piece
+// + head within the group; a tile is tile_rows of them (8, 16, 32 or 128), a piece
 // a run of the pages that the tile sees.  A work item is one piece of one
 // tile, for every K/V head.
 struct Kv4PlanHeader {
@@ -59,7 +59,7 @@ inline Kv4PlanLayout kv4_plan_layout(int num_requests, int64_t num_tokens, int h
     const int64_t group = heads / kv_heads;
     const int64_t rows = num_tokens * group;
     const int64_t mean = num_requests > 0 ? (rows + num_requests - 1) / num_requests : 0;
-    L.tile_rows = mean <= 8 ? 8 : mean <= 16 ? 16 : 32;
+    L.tile_rows = mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 96 ? 32 : 128;
     const int64_t tiles = rows / L.tile_rows + num_requests;
     // twice as many pieces as blocks run at a time (4 per SM, one K/V head each),
     // so that blocks of unequal work even out

@@ -1,0 +1,445 @@
+// f3s_kv4_prefill.cu -- causal attention over request pages for many new tokens:
+// tiles of 128 query rows on tcgen05, K and V held in 4 bits.  (f3s_kv4_math.cuh
+// has the formulas.)
+//
+// A block takes one work item (128 rows of a request and K/V head, a run of its
+// pages) in steps of 64 tokens:
+//   warps 4-7  unpack one page each: codes become fp16 (one AND per two values) in
+//              shared memory, K as [token][channel], V as [channel][token], both in
+//              the 128-byte swizzle; the scales go into arrays per token
+//   warp 8     issues S = Q K^T into one of two S buffers in tensor memory, and
+//              O += P V with P read from tensor memory
+//   warps 0-3  a thread per query row: scores, reference, weights; P (fp16) takes
+//              the place of S.  No row needs another thread's numbers.
+// S of a step runs while the weights of the one before are worked out, and two
+// blocks share an SM.  A weight's reference moves when it passes 2^8; then the
+// row's warp rescales O in tensor memory itself, once the products before are done.
+//
+// V's rows are ordered so that unpacking does not collide in shared memory's
+// banks: row r holds channel (r % 8) * D / 8 + r / 8.
+//
+// Bound: the weights (6 instructions per score of a row, 4 warps), then the
+// products (128 x 64 x D twice per step).
+#include <algorithm>
+#include "f3s_kv4_attend.cuh"
+#include "f3s_tcgen05.cuh"
+
+namespace f3s {
+
+constexpr int kTileRows = 128;
+constexpr int kStepTokens = 64;
+constexpr int kTileThreads = 9 * 32;
+
+template <int D>
+struct TileCfg {
+    static constexpr int RB = kv4_record_bytes(D);
+    static constexpr int ATOMS = D / 64;             // 128-byte column blocks of Q and K
+    static constexpr int Q_BYTES = ATOMS * kTileRows * 128;
+    static constexpr int K_BYTES = ATOMS * kStepTokens * 128;
+    static constexpr int V_BYTES = D * 128;
+    static constexpr int Q = 0;
+    static constexpr int K = Q + Q_BYTES;            // two buffers
+    static constexpr int V = K + 2 * K_BYTES;        // two buffers
+    static constexpr int TOKENS = V + 2 * V_BYTES;   // two buffers of [f, z, l, ri, y][64]
+    static constexpr int TOKEN_BYTES = 5 * kStepTokens * 4;
+    static constexpr int BARS = TOKENS + 2 * TOKEN_BYTES;
+    static constexpr int NBARS = 9;
+    static constexpr int TMEM_SLOT = BARS + (NBARS * 8 + 15) / 16 * 16;
+    static constexpr int SMEM = TMEM_SLOT + 16 + 1024;  // and room to align the base
+    static constexpr int TMEM_COLUMNS = 256;         // S 2 x 64, O D
+};
+
+template <int D, bool PRECISE>
+__global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendParams p) {
+    using C = TileCfg<D>;
+    constexpr int RB = C::RB, W = D / 32;
+    extern __shared__ __align__(1024) uint8_t raw_smem[];
+    uint8_t* smem = raw_smem + ((1024u - (smem_addr(raw_smem) & 1023u)) & 1023u);
+    const uint32_t base = smem_addr(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t kv_full = base + C::BARS, kv_empty = kv_full + 16, s_full = kv_empty + 16, p_full = s_full + 16,
+                   q_full = p_full + 16;
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(kv_full + 8 * i, 128);
+            mbar_init(kv_empty + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1);
+            mbar_init(p_full + 8 * i, 128);
+        }
+        mbar_init(q_full, 128);
+        fence_mbar_init();
+    }
+    if (warp == 8) tmem_alloc(base + C::TMEM_SLOT, C::TMEM_COLUMNS);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *reinterpret_cast<const uint32_t*>(smem + C::TMEM_SLOT);
+    const uint32_t tmem_o = tmem + 128;
+    launch_dependents();
+    wait_for_primary();  // the plan
+    const int item = blockIdx.x / p.kv_heads, hk = blockIdx.x - item * p.kv_heads;
+    const bool live = item < p.plan->num_items;
+    Kv4Item it{};
+    if (live) {
+        const int4* src = reinterpret_cast<const int4*>(reinterpret_cast<const Kv4Item*>(p.plan + 1) + item);
+        const int4 a = src[0], b = src[1];
+        it.request = a.x;
+        it.q_token = a.y;
+        it.row0 = a.z;
+        it.rows = a.w;
+        it.context = b.x;
+        it.page0 = b.y;
+        it.page1 = b.z;
+        it.slot = b.w;
+    }
+    const int steps = live ? (max(it.page1 - it.page0, 0) + 3) / 4 : 0;
+    const int last_row = min(it.row0 + kTileRows, it.rows) - 1;
+    bool ok = true;  // false: a wait ran out; the warp stops waiting
+
+    if (warp < 4 && live) {
+        // ------------------------------------------------------------ rows
+        const int r = threadIdx.x, row = it.row0 + r;
+        const bool valid = row < it.rows;
+        const int at = min(row, last_row), tok = at / p.group;
+        const int limit = it.context + tok;  // the last token this row sees
+        const int64_t out_row = (int64_t)(it.q_token + tok) * p.heads + hk * p.group + at - tok * p.group;
+        // Q as fp16 times a power of two that brings the row's largest to [2^9, 2^10);
+        // channels whose codes come in units of 2^-24 another 2^4
+        float qs = 0.f, unit_scale;
+        {
+            const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
+                                                              (int64_t)(it.q_token + tok) * p.q_token +
+                                                              (int64_t)(hk * p.group + at - tok * p.group) * p.q_head);
+            float amax = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float2 x = q_floats(u[n], p.q_bf16);
+                    if (fabsf(x.x) < INFINITY) amax = fmaxf(amax, fabsf(x.x));  // NaN and infinities stay what they are
+                    if (fabsf(x.y) < INFINITY) amax = fmaxf(amax, fabsf(x.y));
+                }
+            }
+            const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
+            const int up = min(max(9 - e, -120), 120);  // 2^(9 - floor(log2 amax)), within fp32's normal range
+            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+            unit_scale = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;  // 2^20: the codes' unit
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+                const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
+                const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+                uint32_t h[4];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const float2 x = q_floats(u[n], p.q_bf16);
+                    const float m = n & 1 ? f : f * 16.f;
+                    h[n] = pack_half2(x.x * m, x.y * m);
+                    const float2 y = half2_floats(h[n]);
+                    qs += (y.x + y.y) * (n & 1 ? 1.f : 0.0625f);
+                }
+                *reinterpret_cast<uint4*>(smem + C::Q + (c / 8) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
+                    make_uint4(h[0], h[1], h[2], h[3]);
+            }
+            qs *= 9.5367431640625e-7f;  // 2^-20
+        }
+        fence_proxy_async_shared();
+        mbar_arrive(q_full);
+        const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lanes 32 warp ...
+        const uint64_t scale2 = pair(unit_scale, unit_scale), qs2 = pair(qs, qs);
+        float minus_ref = 0.f;
+        uint64_t den = 0, off = 0;
+        bool unset = true;
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            ok = phase_wait(s_full + 8 * b, j >> 1 & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES);
+            const int tok0 = (it.page0 + 4 * j) * 16;
+            uint64_t x[kStepTokens / 2];  // scores less the reference
+            const uint64_t mref2 = pair(minus_ref, minus_ref);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t s[32];
+                tmem_load32(mine + 64 * b + 32 * h, s);
+                tc_wait_ld();
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    const ulonglong2 f = reinterpret_cast<const ulonglong2*>(tokens)[8 * h + c];
+                    const ulonglong2 z = reinterpret_cast<const ulonglong2*>(tokens + 64)[8 * h + c];
+                    const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[8 * h + c];
+                    // scale s (q . u - z sum(q)) + log2 r - R
+                    const uint64_t s0 = pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1]));
+                    const uint64_t s1 = pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]));
+                    x[16 * h + 2 * c] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, s0), add2(l.x, mref2));
+                    x[16 * h + 2 * c + 1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, s1), add2(l.y, mref2));
+                }
+            }
+            // the tile's first row sees the least
+            const bool masked = tok0 + kStepTokens > it.context + (it.row0 + 32 * warp) / p.group + 1;
+            if (masked) {
+#pragma unroll
+                for (int c = 0; c < kStepTokens / 2; ++c) {
+                    float2 y = unpair(x[c]);
+                    if (tok0 + 2 * c > limit) y.x = -INFINITY;
+                    if (tok0 + 2 * c + 1 > limit) y.y = -INFINITY;
+                    x[c] = pair(y.x, y.y);
+                }
+            }
+            bool over = unset;
+#pragma unroll
+            for (int c = 0; c < kStepTokens / 2; ++c) {
+                const float2 y = unpair(x[c]);
+                over = over || y.x > kRescaleAt || y.y > kRescaleAt;
+            }
+            if (__any_sync(0xffffffffu, over)) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < kStepTokens / 2; ++c) {
+                    const float2 y = unpair(x[c]);
+                    m = fmaxf(m, fmaxf(y.x, y.y));
+                }
+                float up, down = 1.f;  // the reference moves up by `up`
+                if (unset) {           // nothing seen so far: the sums are 0, whatever they are scaled by
+                    up = m > -INFINITY ? m : 0.f;
+                    if (m > -INFINITY) unset = false;
+                } else {
+                    up = fmaxf(m, 0.f);
+                    down = exp2_approx(-up);
+                }
+                minus_ref -= up;
+                den = mul2(den, pair(down, down));
+                off = mul2(off, pair(down, down));
+#pragma unroll
+                for (int c = 0; c < kStepTokens / 2; ++c) x[c] = add2(x[c], pair(-up, -up));
+                if (j > 0) {
+                    // O, once the products so far are in it
+                    ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t o[32];
+                        tmem_load32(mine + 128 + c, o);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
+                        tmem_store32(mine + 128 + c, o);
+                    }
+                }
+            }
+            // weights: P over S, two tokens per column
+            uint32_t hi[32], lo[PRECISE ? 32 : 1];
+#pragma unroll
+            for (int c = 0; c < kStepTokens / 2; ++c) {
+                const float2 y = unpair(x[c]);
+                const float2 a = make_float2(exp2_approx(y.x), exp2_approx(y.y));
+                hi[c] = pack_half2(a.x, a.y);
+                if constexpr (PRECISE) {
+                    const float2 h = half2_floats(hi[c]);
+                    lo[c] = pack_half2(a.x - h.x, a.y - h.y);
+                }
+                x[c] = pair(a.x, a.y);
+            }
+            __syncwarp();
+            tmem_store32(mine + 64 * b, hi);
+            if constexpr (PRECISE) tmem_store32(mine + 64 * b + 32, lo);
+            if (masked) {
+                // a hidden token's scale and zero may be anything, NaN too
+                float2 d = unpair(den), o = unpair(off);
+#pragma unroll
+                for (int c = 0; c < kStepTokens / 2; ++c) {
+                    const float2 a = unpair(x[c]);
+                    if (tok0 + 2 * c <= limit) {
+                        d.x = fmaf(a.x, tokens[192 + 2 * c], d.x);
+                        o.x = fmaf(a.x, tokens[256 + 2 * c], o.x);
+                    }
+                    if (tok0 + 2 * c + 1 <= limit) {
+                        d.y = fmaf(a.y, tokens[192 + 2 * c + 1], d.y);
+                        o.y = fmaf(a.y, tokens[256 + 2 * c + 1], o.y);
+                    }
+                }
+                den = pair(d.x, d.y);
+                off = pair(o.x, o.y);
+            } else {
+#pragma unroll
+                for (int c = 0; c < kStepTokens / 4; ++c) {
+                    const ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[c];
+                    const ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[c];
+                    den = fma2(x[2 * c + 1], ri.y, fma2(x[2 * c], ri.x, den));
+                    off = fma2(x[2 * c + 1], y.y, fma2(x[2 * c], y.x, off));
+                }
+            }
+            tc_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_full + 8 * b);
+        }
+        // ---- the result
+        if (ok && steps > 0) {
+            ok = phase_wait(kv_empty + 8 * ((steps - 1) & 1), (steps - 1) >> 1 & 1, p.status);
+            tc_fence_after();
+        }
+        const float2 d2 = unpair(den), o2 = unpair(off);
+        const float row_den = d2.x + d2.y, row_off = o2.x + o2.y;
+        const float inv = it.slot >= 0 ? 1.f : row_den != 0.f ? __frcp_rn(row_den) : 0.f;
+        float* part = it.slot >= 0 ? p.partials + ((int64_t)it.slot * p.kv_heads + hk) * kTileRows * (D + 2) : nullptr;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+            uint32_t o[32] = {};
+            __syncwarp();
+            if (steps > 0) {
+                tmem_load32(mine + 128 + c, o);
+                tc_wait_ld();
+            }
+            if (!valid) continue;
+            // column c + 8 i + g holds channel g * D / 8 + c / 8 + i, its codes in units of
+            // 2^-24 (even i) and 2^-20
+#pragma unroll
+            for (int g = 0; g < 8; ++g) {
+                float v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    v[i] = fmaf(__uint_as_float(o[8 * i + g]), i & 1 ? 1048576.f : 16777216.f, -row_off) * inv;
+                if (part) *reinterpret_cast<float4*>(part + r * D + g * (D / 8) + c / 8) = make_float4(v[0], v[1], v[2], v[3]);
+                else store_channels<4>(p.o, out_row * D + g * (D / 8) + c / 8, v, p.o_dtype);
+            }
+        }
+        if (part && valid)
+            *reinterpret_cast<float2*>(part + kTileRows * D + 2 * r) = make_float2(unset ? kNoReference : -minus_ref, row_den);
+        tc_fence_before();
+    } else if (warp < 8 && live) {
+        // ------------------------------------------------------------ codes
+        const int dw = warp - 4, g = lane >> 2, t = lane & 3;
+        const int64_t page_bytes = (int64_t)p.kv_heads * RB;
+        const int* list = p.tables + (int64_t)it.request * p.table_stride;
+        const int last_seen = it.context + last_row / p.group;
+        auto id_of = [&](int j) {
+            const int page = it.page0 + 4 * j + dw;
+            int id = page < it.page1 ? list[page] : -1;
+            if (id < -1 || id >= p.num_pages) {
+                atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
+                id = -1;
+            }
+            return id;
+        };
+        uint32_t kg[W], kh[W], v0[W], v1[W];
+        uint2 sc;
+        auto load = [&](int id) {
+            const uint8_t* rec = p.pages + (int64_t)max(id, 0) * page_bytes + (int64_t)hk * RB;
+            lds_words<W>(rec + g * (D / 2) + t * (D / 8), kg);
+            lds_words<W>(rec + (g + 8) * (D / 2) + t * (D / 8), kh);
+            lds_words<W>(rec + 8 * D + lane * (D / 8), v0);
+            lds_words<W>(rec + 12 * D + lane * (D / 8), v1);
+            sc = *reinterpret_cast<const uint2*>(rec + kv4_scale_off(D, lane & 15));
+        };
+        int id = steps > 0 ? id_of(0) : -1, id_next = steps > 1 ? id_of(1) : -1;
+        if (steps > 0) load(id);
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            ok = phase_wait(kv_empty + 8 * b, (j >> 1 & 1) ^ 1, p.status);
+            if (!ok) break;
+            uint8_t* ks = smem + C::K + b * C::K_BYTES;
+            uint8_t* vs = smem + C::V + b * C::V_BYTES;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                const int chunk = t * W + w;  // of 8 channels
+                const uint32_t g8 = kg[w] >> 8, h8 = kh[w] >> 8;
+                uint8_t* dst = ks + (chunk / 8) * (kStepTokens * 128) + (dw * 16 + g) * 128 + (((chunk & 7) ^ g) << 4);
+                *reinterpret_cast<uint4*>(dst) = make_uint4(kg[w] & kNib0, kg[w] & kNib1, g8 & kNib0, g8 & kNib1);
+                *reinterpret_cast<uint4*>(dst + 8 * 128) = make_uint4(kh[w] & kNib0, kh[w] & kNib1, h8 & kNib0, h8 & kNib1);
+                const uint32_t a8 = v0[w] >> 8, b8 = v1[w] >> 8;
+                const uint32_t an[4] = {v0[w] & kNib0, v0[w] & kNib1, a8 & kNib0, a8 & kNib1};
+                const uint32_t bn[4] = {v1[w] & kNib0, v1[w] & kNib1, b8 & kNib0, b8 & kNib1};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    uint8_t* to = vs + ((4 * w + n) * 8 + g) * 128 + 4 * t;
+                    *reinterpret_cast<uint32_t*>(to + (((2 * dw) ^ g) << 4)) = an[n];
+                    *reinterpret_cast<uint32_t*>(to + (((2 * dw + 1) ^ g) << 4)) = bn[n];
+                }
+            }
+            if (lane < 16) {
+                float* tokens = reinterpret_cast<float*>(smem + C::TOKENS + b * C::TOKEN_BYTES) + dw * 16 + lane;
+                const float2 k2 = half2_floats(sc.x), v2 = half2_floats(sc.y);
+                const float r = v2.x < kKv4MinScale ? kKv4MinScale : v2.x;  // keeps a NaN
+                // tokens that no row of the tile sees weigh nothing, whatever is there
+                const bool hidden = id < 0 || (it.page0 + 4 * j + dw) * 16 + lane > last_seen;
+                tokens[0] = hidden ? 0.f : k2.x;
+                tokens[64] = hidden ? 0.f : -k2.y;
+                tokens[128] = hidden ? -INFINITY : log2_approx(r);
+                tokens[192] = hidden ? 0.f : rcp_approx(r);
+                tokens[256] = hidden ? 0.f : v2.y;
+            }
+            id = id_next;
+            if (j + 1 < steps) load(id);
+            if (j + 2 < steps) id_next = id_of(j + 2);
+            fence_proxy_async_shared();
+            mbar_arrive(kv_full + 8 * b);
+        }
+    } else if (warp == 8 && live && steps > 0) {
+        // ------------------------------------------------------------ products
+        ok = phase_wait(q_full, 0, p.status);
+        auto weigh = [&](int j) {  // O += P V of step j
+            const int b = j & 1;
+            ok = phase_wait(p_full + 8 * b, j >> 1 & 1, p.status);
+            if (!ok) return;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < kStepTokens / 16; ++k) {
+                    const uint64_t v = smem_operand(base + C::V + b * C::V_BYTES + 32 * k);
+                    mma_ts(tmem_o, tmem + 64 * b + 8 * k, v, mma_f16_shape(kTileRows, D), j > 0 || k > 0);
+                    if constexpr (PRECISE) mma_ts(tmem_o, tmem + 64 * b + 32 + 8 * k, v, mma_f16_shape(kTileRows, D), true);
+                }
+                mma_commit(kv_empty + 8 * b);  // K, V, the tokens' numbers and P are free, O is the step's
+            }
+            __syncwarp();
+        };
+        for (int j = 0; j < steps && ok; ++j) {
+            const int b = j & 1;
+            ok = phase_wait(kv_full + 8 * b, j >> 1 & 1, p.status);
+            if (!ok) break;
+            tc_fence_after();
+            if (lane == 0) {
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(tmem + 64 * b, smem_operand(base + C::Q + (k / 4) * (kTileRows * 128) + 32 * (k % 4)),
+                           smem_operand(base + C::K + b * C::K_BYTES + (k / 4) * (kStepTokens * 128) + 32 * (k % 4)),
+                           mma_f16_shape(kTileRows, kStepTokens), k > 0);
+                mma_commit(s_full + 8 * b);
+            }
+            __syncwarp();
+            if (j > 0) weigh(j - 1);
+        }
+        if (ok) weigh(steps - 1);
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        tmem_free(tmem, C::TMEM_COLUMNS);
+    }
+}
+
+template <int D, bool PRECISE>
+static int tiles_variant(const AttendParams& p, int64_t units, cudaStream_t stream) {
+    using C = TileCfg<D>;
+    static PerContext<int> attr;
+    const int rc = attr.get(nullptr, [](int* v) -> int {
+        *v = 1;
+        F3S_CUDA_TRY(cudaFuncSetAttribute(k_attend4_tiles<D, PRECISE>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+        return F3S_SUCCESS;
+    });
+    if (rc != F3S_SUCCESS) return rc;
+    if (units > INT32_MAX) return F3S_ERR_TOO_LARGE;
+    if (units == 0) return F3S_SUCCESS;
+    return launch_after(k_attend4_tiles<D, PRECISE>, (unsigned)units, kTileThreads, C::SMEM, stream, p);
+}
+
+int attend_tiles128(const AttendParams& p, int head_dim, int64_t units, cudaStream_t stream) {
+    const bool precise = p.o_dtype == F3S_OUT_F32;
+    if (head_dim == 64) return precise ? tiles_variant<64, true>(p, units, stream) : tiles_variant<64, false>(p, units, stream);
+    return precise ? tiles_variant<128, true>(p, units, stream) : tiles_variant<128, false>(p, units, stream);
+}
+
+}  // namespace f3s
