@@ -261,8 +261,9 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
                 const BtRequest& w = s_req[i];
                 const int m = (w.pages + piece - 1) / piece;
                 const int local = (int)(it - s_item[i]);
-                const int tile = local / m, part = local - tile * m;
-                const int row0 = tile * p.tile_rows, rows = w.count * p.group;
+                const int nth = local / m, part = local - nth * m;
+                // a request's last rows see the most: their tiles begin first
+                const int row0 = (w.tiles - 1 - nth) * p.tile_rows, rows = w.count * p.group;
                 const int last = min(row0 + p.tile_rows, rows) - 1;  // the tile's last row sees the most
                 const int seen = (w.context + last / p.group) / 16 + 1;
                 Kv4Item d;
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
                 d.slot = m > 1 && slot < (uint32_t)p.slots_cap ? (int)slot : -1;
                 p.items[it] = d;
                 if (part == 0 && m > 1) {
-                    const uint32_t sp = s_split[i] + tile;
+                    const uint32_t sp = s_split[i] + nth;
                     if (sp < (uint32_t)p.splits_cap) {
                         Kv4Split s{};
                         s.slot = (int)slot;

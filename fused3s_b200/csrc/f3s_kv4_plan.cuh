@@ -61,9 +61,9 @@ inline Kv4PlanLayout kv4_plan_layout(int num_requests, int64_t num_tokens, int h
     const int64_t mean = num_requests > 0 ? (rows + num_requests - 1) / num_requests : 0;
     L.tile_rows = mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 96 ? 32 : 128;
     const int64_t tiles = rows / L.tile_rows + num_requests;
-    // twice as many pieces as blocks run at a time (4 per SM, one K/V head each),
+    // twice as many pieces as blocks run at a time (4 per SM, 2 of 128 rows, one K/V head each),
     // so that blocks of unequal work even out
-    L.target = (int)std::max<int64_t>(1, (int64_t)sms * 8 / kv_heads);
+    L.target = (int)std::max<int64_t>(1, (int64_t)sms * (L.tile_rows == 128 ? 4 : 8) / kv_heads);
     L.items_cap = tiles + L.target;
     L.slots_cap = 2 * (int64_t)L.target;
     L.splits_cap = L.target;

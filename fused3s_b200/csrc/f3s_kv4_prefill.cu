@@ -21,6 +21,7 @@
 // Bound: the weights (6 instructions per score of a row, 4 warps), then the
 // products (128 x 64 x D twice per step).
 #include <algorithm>
+#include <type_traits>
 #include "f3s_kv4_attend.cuh"
 #include "f3s_tcgen05.cuh"
 
@@ -159,64 +160,83 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             tc_fence_after();
             const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES);
             const int tok0 = (it.page0 + 4 * j) * 16;
-            uint64_t x[kStepTokens / 2];  // scores less the reference
-            const uint64_t mref2 = pair(minus_ref, minus_ref);
+            uint32_t hi[32], lo[PRECISE ? 32 : 1];  // P, two tokens each, and what its rounding drops
+            // Weights and sums against the reference as it stands; the largest score
+            // over it.  In one run of instructions per 32 scores: nothing is kept of S.
+            auto weigh_row = [&](auto hides, uint64_t& den_out, uint64_t& off_out) {
+                constexpr bool HIDES = decltype(hides)::value;
+                float most = -INFINITY;
+                uint64_t d = den, o = off;
+                const uint64_t mref2 = pair(minus_ref, minus_ref);
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                uint32_t s[32];
-                tmem_load32(mine + 64 * b + 32 * h, s);
-                tc_wait_ld();
+                for (int h = 0; h < 2; ++h) {
+                    uint32_t s[32];
+                    tmem_load32(mine + 64 * b + 32 * h, s);
+                    tc_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    const ulonglong2 f = reinterpret_cast<const ulonglong2*>(tokens)[8 * h + c];
-                    const ulonglong2 z = reinterpret_cast<const ulonglong2*>(tokens + 64)[8 * h + c];
-                    const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[8 * h + c];
-                    // scale s (q . u - z sum(q)) + log2 r - R
-                    const uint64_t s0 = pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1]));
-                    const uint64_t s1 = pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]));
-                    x[16 * h + 2 * c] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, s0), add2(l.x, mref2));
-                    x[16 * h + 2 * c + 1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, s1), add2(l.y, mref2));
+                    for (int c = 0; c < 8; ++c) {
+                        const ulonglong2 f = reinterpret_cast<const ulonglong2*>(tokens)[8 * h + c];
+                        const ulonglong2 z = reinterpret_cast<const ulonglong2*>(tokens + 64)[8 * h + c];
+                        const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[8 * h + c];
+                        ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[8 * h + c];
+                        ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[8 * h + c];
+                        // scale s (q . u - z sum(q)) + log2 r - R
+                        uint64_t x[2] = {pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])),
+                                         pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]))};
+                        x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), add2(l.x, mref2));
+                        x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), add2(l.y, mref2));
+                        if constexpr (HIDES) {
+                            // a hidden token's scale and zero may be anything, NaN too
+                            const int at_token = tok0 + 32 * h + 4 * c;
+                            auto keep = [](uint64_t v, bool a, bool c2, float other) {
+                                const float2 w = unpair(v);
+                                return pair(a ? w.x : other, c2 ? w.y : other);
+                            };
+                            const bool k0 = at_token <= limit, k1 = at_token + 1 <= limit, k2 = at_token + 2 <= limit,
+                                       k3 = at_token + 3 <= limit;
+                            x[0] = keep(x[0], k0, k1, -INFINITY);
+                            x[1] = keep(x[1], k2, k3, -INFINITY);
+                            ri.x = keep(ri.x, k0, k1, 0.f);
+                            ri.y = keep(ri.y, k2, k3, 0.f);
+                            y.x = keep(y.x, k0, k1, 0.f);
+                            y.y = keep(y.y, k2, k3, 0.f);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float2 v = unpair(x[i]);
+                            most = fmaxf(most, fmaxf(v.x, v.y));
+                            const float2 a = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                            const uint64_t a2 = pair(a.x, a.y);
+                            const uint32_t packed = pack_half2(a.x, a.y);
+                            hi[16 * h + 2 * c + i] = packed;
+                            if constexpr (PRECISE) {
+                                const float2 w = half2_floats(packed);
+                                lo[16 * h + 2 * c + i] = pack_half2(a.x - w.x, a.y - w.y);
+                            }
+                            d = fma2(a2, i ? ri.y : ri.x, d);
+                            o = fma2(a2, i ? y.y : y.x, o);
+                        }
+                    }
                 }
-            }
-            // the tile's first row sees the least
-            const bool masked = tok0 + kStepTokens > it.context + (it.row0 + 32 * warp) / p.group + 1;
-            if (masked) {
-#pragma unroll
-                for (int c = 0; c < kStepTokens / 2; ++c) {
-                    float2 y = unpair(x[c]);
-                    if (tok0 + 2 * c > limit) y.x = -INFINITY;
-                    if (tok0 + 2 * c + 1 > limit) y.y = -INFINITY;
-                    x[c] = pair(y.x, y.y);
-                }
-            }
-            bool over = unset;
-#pragma unroll
-            for (int c = 0; c < kStepTokens / 2; ++c) {
-                const float2 y = unpair(x[c]);
-                over = over || y.x > kRescaleAt || y.y > kRescaleAt;
-            }
-            if (__any_sync(0xffffffffu, over)) {
-                float m = -INFINITY;
-#pragma unroll
-                for (int c = 0; c < kStepTokens / 2; ++c) {
-                    const float2 y = unpair(x[c]);
-                    m = fmaxf(m, fmaxf(y.x, y.y));
-                }
-                float up, down = 1.f;  // the reference moves up by `up`
-                if (unset) {           // nothing seen so far: the sums are 0, whatever they are scaled by
-                    up = m > -INFINITY ? m : 0.f;
-                    if (m > -INFINITY) unset = false;
-                } else {
-                    up = fmaxf(m, 0.f);
-                    down = exp2_approx(-up);
-                }
+                den_out = d;
+                off_out = o;
+                return most;
+            };
+            // the warp's first row sees the least
+            const bool hides = tok0 + kStepTokens > it.context + (it.row0 + 32 * warp) / p.group + 1;
+            uint64_t den_new, off_new;
+            for (;;) {
+                const float most = hides ? weigh_row(std::true_type{}, den_new, off_new)
+                                         : weigh_row(std::false_type{}, den_new, off_new);
+                // a row that has seen nothing takes its first largest score as the reference
+                if (!__any_sync(0xffffffffu, unset ? most > -INFINITY : most > kRescaleAt)) break;
+                const float up = unset ? (most > -INFINITY ? most : 0.f) : fmaxf(most, 0.f);  // the reference moves up by this
+                const float down = unset ? 1.f : exp2_approx(-up);
+                unset = unset && !(most > -INFINITY);
                 minus_ref -= up;
                 den = mul2(den, pair(down, down));
                 off = mul2(off, pair(down, down));
-#pragma unroll
-                for (int c = 0; c < kStepTokens / 2; ++c) x[c] = add2(x[c], pair(-up, -up));
-                if (j > 0) {
-                    // O, once the products so far are in it
+                if (j > 0) {  // O, once the products so far are in it
                     ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status);
                     tc_fence_after();
 #pragma unroll 1
@@ -228,50 +248,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * down);
                         tmem_store32(mine + 128 + c, o);
                     }
+                    tc_wait_st();
                 }
             }
-            // weights: P over S, two tokens per column
-            uint32_t hi[32], lo[PRECISE ? 32 : 1];
-#pragma unroll
-            for (int c = 0; c < kStepTokens / 2; ++c) {
-                const float2 y = unpair(x[c]);
-                const float2 a = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                hi[c] = pack_half2(a.x, a.y);
-                if constexpr (PRECISE) {
-                    const float2 h = half2_floats(hi[c]);
-                    lo[c] = pack_half2(a.x - h.x, a.y - h.y);
-                }
-                x[c] = pair(a.x, a.y);
-            }
+            den = den_new;
+            off = off_new;
             __syncwarp();
             tmem_store32(mine + 64 * b, hi);
             if constexpr (PRECISE) tmem_store32(mine + 64 * b + 32, lo);
-            if (masked) {
-                // a hidden token's scale and zero may be anything, NaN too
-                float2 d = unpair(den), o = unpair(off);
-#pragma unroll
-                for (int c = 0; c < kStepTokens / 2; ++c) {
-                    const float2 a = unpair(x[c]);
-                    if (tok0 + 2 * c <= limit) {
-                        d.x = fmaf(a.x, tokens[192 + 2 * c], d.x);
-                        o.x = fmaf(a.x, tokens[256 + 2 * c], o.x);
-                    }
-                    if (tok0 + 2 * c + 1 <= limit) {
-                        d.y = fmaf(a.y, tokens[192 + 2 * c + 1], d.y);
-                        o.y = fmaf(a.y, tokens[256 + 2 * c + 1], o.y);
-                    }
-                }
-                den = pair(d.x, d.y);
-                off = pair(o.x, o.y);
-            } else {
-#pragma unroll
-                for (int c = 0; c < kStepTokens / 4; ++c) {
-                    const ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[c];
-                    const ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[c];
-                    den = fma2(x[2 * c + 1], ri.y, fma2(x[2 * c], ri.x, den));
-                    off = fma2(x[2 * c + 1], y.y, fma2(x[2 * c], y.x, off));
-                }
-            }
             tc_wait_st();
             tc_fence_before();
             mbar_arrive(p_full + 8 * b);
