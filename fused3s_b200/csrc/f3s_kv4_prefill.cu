@@ -4,22 +4,26 @@
 //
 // A block takes one work item (128 rows of a request and K/V head, a run of its
 // pages) in steps of 64 tokens:
-//   warps 4-7  unpack one page each: codes become fp16 (one AND per two values) in
-//              shared memory, K as [token][channel], V as [channel][token], both in
-//              the 128-byte swizzle; the scales go into arrays per token
-//   warp 8     issues S = Q K^T into one of two S buffers in tensor memory, and
-//              O += P V with P read from tensor memory
-//   warps 0-3  a thread per query row: scores, reference, weights; P (fp16) takes
-//              the place of S.  No row needs another thread's numbers.
+//   warps 0-7   two threads per query row, 32 tokens of the step each: scores,
+//               weights; P (fp16) takes the place of S.  The two agree on the row's
+//               reference by a barrier that also votes.
+//   warps 8-11  unpack one page each: codes become fp16 (one AND per two values) in
+//               shared memory, K as [token][channel], V as [channel][token], both in
+//               the 128-byte swizzle; the scales go into arrays per token
+//   warp 12     issues S = Q K^T into one of two S buffers in tensor memory, and
+//               O += P V with P read from tensor memory
 // S of a step runs while the weights of the one before are worked out, and two
 // blocks share an SM.  A weight's reference moves when it passes 2^8; then the
-// row's warp rescales O in tensor memory itself, once the products before are done.
+// rows' warps rescale O in tensor memory themselves, once the products before are
+// done.
 //
 // V's rows are ordered so that unpacking does not collide in shared memory's
 // banks: row r holds channel (r % 8) * D / 8 + r / 8.
 //
-// Bound: the weights (6 instructions per score of a row, 4 warps), then the
-// products (128 x 64 x D twice per step).
+// Bound: the weights (13 instructions and 2.5 loads from shared memory per two
+// scores), then the products (128 x 64 x D twice per step).  One thread per row with
+// 64 tokens took 316 us where two take 255 us (prompts of 147 GFLOP;
+// mma.sync with 32 rows took 506).
 #include <algorithm>
 #include <type_traits>
 #include "f3s_kv4_attend.cuh"
@@ -29,7 +33,9 @@ namespace f3s {
 
 constexpr int kTileRows = 128;
 constexpr int kStepTokens = 64;
-constexpr int kTileThreads = 9 * 32;
+constexpr int kRowWarps = 8;   // two halves of a step's tokens x 4 x 32 rows
+constexpr int kCodeWarps = 4;  // a page each
+constexpr int kTileThreads = (kRowWarps + kCodeWarps + 1) * 32;
 
 template <int D>
 struct TileCfg {
@@ -43,7 +49,8 @@ struct TileCfg {
     static constexpr int V = K + 2 * K_BYTES;        // two buffers
     static constexpr int TOKENS = V + 2 * V_BYTES;   // two buffers of [f, z, l, ri, y][64]
     static constexpr int TOKEN_BYTES = 5 * kStepTokens * 4;
-    static constexpr int BARS = TOKENS + 2 * TOKEN_BYTES;
+    static constexpr int ROWS = TOKENS + 2 * TOKEN_BYTES;  // [unit scale, sum q][128], [largest, den, off][half][128]
+    static constexpr int BARS = ROWS + 8 * kTileRows * 4;
     static constexpr int NBARS = 9;
     static constexpr int TMEM_SLOT = BARS + (NBARS * 8 + 15) / 16 * 16;
     static constexpr int SMEM = TMEM_SLOT + 16 + 1024;  // and room to align the base
@@ -66,12 +73,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             mbar_init(kv_full + 8 * i, 128);
             mbar_init(kv_empty + 8 * i, 1);
             mbar_init(s_full + 8 * i, 1);
-            mbar_init(p_full + 8 * i, 128);
+            mbar_init(p_full + 8 * i, kRowWarps * 32);
         }
         mbar_init(q_full, 128);
         fence_mbar_init();
     }
-    if (warp == 8) tmem_alloc(base + C::TMEM_SLOT, C::TMEM_COLUMNS);
+    if (warp == kRowWarps + kCodeWarps) tmem_alloc(base + C::TMEM_SLOT, C::TMEM_COLUMNS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -98,21 +105,32 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
     const int last_row = min(it.row0 + kTileRows, it.rows) - 1;
     bool ok = true;  // false: a wait ran out; the warp stops waiting
 
-    if (warp < 4 && live) {
+    if (warp < kRowWarps && live) {
         // ------------------------------------------------------------ rows
-        const int r = threadIdx.x, row = it.row0 + r;
+        const int half = warp >> 2, quad = warp & 3;  // tokens 32 half ... of a step; rows 32 quad ...
+        const int r = quad * 32 + lane, row = it.row0 + r;
         const bool valid = row < it.rows;
         const int at = min(row, last_row), tok = at / p.group;
         const int limit = it.context + tok;  // the last token this row sees
         const int64_t out_row = (int64_t)(it.q_token + tok) * p.heads + hk * p.group + at - tok * p.group;
+        float* rows = reinterpret_cast<float*>(smem + C::ROWS);
+        auto pair_sync = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + quad) : "memory"); };
+        auto pair_any = [&](bool x) {
+            uint32_t any;
+            asm volatile(
+                "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %2, 0;\n\tbar.red.or.pred b, %1, 64, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+                : "=r"(any)
+                : "r"(1 + quad), "r"((uint32_t)x)
+                : "memory");
+            return any != 0;
+        };
         // Q as fp16 times a power of two that brings the row's largest to [2^9, 2^10);
         // channels whose codes come in units of 2^-24 another 2^4
-        float qs = 0.f, unit_scale;
-        {
+        if (half == 0) {
             const uint4* src = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) +
                                                               (int64_t)(it.q_token + tok) * p.q_token +
                                                               (int64_t)(hk * p.group + at - tok * p.group) * p.q_head);
-            float amax = 0.f;
+            float amax = 0.f, sum = 0.f;
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
@@ -125,9 +143,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 }
             }
             const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
-            const int up = min(max(9 - e, -120), 120);  // 2^(9 - floor(log2 amax)), within fp32's normal range
+            const int up = min(max(9 - e, -100), 120);  // 2^(9 - floor(log2 amax)), within fp32's normal range
             const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-            unit_scale = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;  // 2^20: the codes' unit
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
                 const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
@@ -139,83 +156,84 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                     const float m = n & 1 ? f : f * 16.f;
                     h[n] = pack_half2(x.x * m, x.y * m);
                     const float2 y = half2_floats(h[n]);
-                    qs += (y.x + y.y) * (n & 1 ? 1.f : 0.0625f);
+                    sum += (y.x + y.y) * (n & 1 ? 1.f : 0.0625f);
                 }
                 *reinterpret_cast<uint4*>(smem + C::Q + (c / 8) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
                     make_uint4(h[0], h[1], h[2], h[3]);
             }
-            qs *= 9.5367431640625e-7f;  // 2^-20
+            rows[r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;  // 2^20: the codes' unit
+            rows[kTileRows + r] = sum * 9.5367431640625e-7f;                              // 2^-20
+            fence_proxy_async_shared();
+            mbar_arrive(q_full);
         }
-        fence_proxy_async_shared();
-        mbar_arrive(q_full);
-        const uint32_t mine = tmem + ((uint32_t)warp << 21);  // lanes 32 warp ...
+        pair_sync();
+        const float unit_scale = rows[r], qs = rows[kTileRows + r];
+        float* largest = rows + 2 * kTileRows;
+        float* sums = rows + 4 * kTileRows;
+        const uint32_t mine = tmem + ((uint32_t)quad << 21);  // lanes 32 quad ...
         const uint64_t scale2 = pair(unit_scale, unit_scale), qs2 = pair(qs, qs);
         float minus_ref = 0.f;
-        uint64_t den = 0, off = 0;
+        uint64_t den = 0, off = 0;  // of this half's tokens
         bool unset = true;
-        for (int j = 0; j < steps && ok; ++j) {
+        for (int j = 0; j < steps; ++j) {
             const int b = j & 1;
-            ok = phase_wait(s_full + 8 * b, j >> 1 & 1, p.status);
-            if (!ok) break;
+            ok = ok && phase_wait(s_full + 8 * b, j >> 1 & 1, p.status);
+            if (pair_any(!ok)) {  // both halves leave together
+                ok = false;
+                break;
+            }
             tc_fence_after();
-            const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES);
-            const int tok0 = (it.page0 + 4 * j) * 16;
-            uint32_t hi[32], lo[PRECISE ? 32 : 1];  // P, two tokens each, and what its rounding drops
-            // Weights and sums against the reference as it stands; the largest score
-            // over it.  In one run of instructions per 32 scores: nothing is kept of S.
+            const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES) + 32 * half;
+            const int tok0 = (it.page0 + 4 * j) * 16 + 32 * half;
+            uint32_t hi[16], lo[PRECISE ? 16 : 1];  // P, two tokens each, and what its rounding drops
+            // Weights and sums against the reference as it stands; the largest score over it
             auto weigh_row = [&](auto hides, uint64_t& den_out, uint64_t& off_out) {
                 constexpr bool HIDES = decltype(hides)::value;
                 float most = -INFINITY;
                 uint64_t d = den, o = off;
                 const uint64_t mref2 = pair(minus_ref, minus_ref);
+                uint32_t s[32];
+                tmem_load32(mine + 64 * b + 32 * half, s);
+                tc_wait_ld();
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t s[32];
-                    tmem_load32(mine + 64 * b + 32 * h, s);
-                    tc_wait_ld();
+                for (int c = 0; c < 8; ++c) {
+                    const ulonglong2 f = reinterpret_cast<const ulonglong2*>(tokens)[c];
+                    const ulonglong2 z = reinterpret_cast<const ulonglong2*>(tokens + 64)[c];
+                    const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[c];
+                    ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[c];
+                    ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[c];
+                    // scale s (q . u - z sum(q)) + log2 r - R
+                    uint64_t x[2] = {pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])),
+                                     pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]))};
+                    x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), add2(l.x, mref2));
+                    x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), add2(l.y, mref2));
+                    if constexpr (HIDES) {
+                        // a hidden token's scale and zero may be anything, NaN too
+                        const int left = limit - (tok0 + 4 * c);  // tokens up to this one are seen
+                        auto keep = [](uint64_t v, bool a, bool c2, float other) {
+                            const float2 w = unpair(v);
+                            return pair(a ? w.x : other, c2 ? w.y : other);
+                        };
+                        x[0] = keep(x[0], left >= 0, left >= 1, -INFINITY);
+                        x[1] = keep(x[1], left >= 2, left >= 3, -INFINITY);
+                        ri.x = keep(ri.x, left >= 0, left >= 1, 0.f);
+                        ri.y = keep(ri.y, left >= 2, left >= 3, 0.f);
+                        y.x = keep(y.x, left >= 0, left >= 1, 0.f);
+                        y.y = keep(y.y, left >= 2, left >= 3, 0.f);
+                    }
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const ulonglong2 f = reinterpret_cast<const ulonglong2*>(tokens)[8 * h + c];
-                        const ulonglong2 z = reinterpret_cast<const ulonglong2*>(tokens + 64)[8 * h + c];
-                        const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[8 * h + c];
-                        ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[8 * h + c];
-                        ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[8 * h + c];
-                        // scale s (q . u - z sum(q)) + log2 r - R
-                        uint64_t x[2] = {pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])),
-                                         pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]))};
-                        x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), add2(l.x, mref2));
-                        x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), add2(l.y, mref2));
-                        if constexpr (HIDES) {
-                            // a hidden token's scale and zero may be anything, NaN too
-                            const int at_token = tok0 + 32 * h + 4 * c;
-                            auto keep = [](uint64_t v, bool a, bool c2, float other) {
-                                const float2 w = unpair(v);
-                                return pair(a ? w.x : other, c2 ? w.y : other);
-                            };
-                            const bool k0 = at_token <= limit, k1 = at_token + 1 <= limit, k2 = at_token + 2 <= limit,
-                                       k3 = at_token + 3 <= limit;
-                            x[0] = keep(x[0], k0, k1, -INFINITY);
-                            x[1] = keep(x[1], k2, k3, -INFINITY);
-                            ri.x = keep(ri.x, k0, k1, 0.f);
-                            ri.y = keep(ri.y, k2, k3, 0.f);
-                            y.x = keep(y.x, k0, k1, 0.f);
-                            y.y = keep(y.y, k2, k3, 0.f);
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 v = unpair(x[i]);
+                        most = fmaxf(most, fmaxf(v.x, v.y));
+                        const float2 a = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                        const uint64_t a2 = pair(a.x, a.y);
+                        hi[2 * c + i] = pack_half2(a.x, a.y);
+                        if constexpr (PRECISE) {
+                            const float2 w = half2_floats(hi[2 * c + i]);
+                            lo[2 * c + i] = pack_half2(a.x - w.x, a.y - w.y);
                         }
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const float2 v = unpair(x[i]);
-                            most = fmaxf(most, fmaxf(v.x, v.y));
-                            const float2 a = make_float2(exp2_approx(v.x), exp2_approx(v.y));
-                            const uint64_t a2 = pair(a.x, a.y);
-                            const uint32_t packed = pack_half2(a.x, a.y);
-                            hi[16 * h + 2 * c + i] = packed;
-                            if constexpr (PRECISE) {
-                                const float2 w = half2_floats(packed);
-                                lo[16 * h + 2 * c + i] = pack_half2(a.x - w.x, a.y - w.y);
-                            }
-                            d = fma2(a2, i ? ri.y : ri.x, d);
-                            o = fma2(a2, i ? y.y : y.x, o);
-                        }
+                        d = fma2(a2, i ? ri.y : ri.x, d);
+                        o = fma2(a2, i ? y.y : y.x, o);
                     }
                 }
                 den_out = d;
@@ -223,24 +241,28 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 return most;
             };
             // the warp's first row sees the least
-            const bool hides = tok0 + kStepTokens > it.context + (it.row0 + 32 * warp) / p.group + 1;
+            const bool hides = tok0 + 32 > it.context + (it.row0 + 32 * quad) / p.group + 1;
             uint64_t den_new, off_new;
             for (;;) {
                 const float most = hides ? weigh_row(std::true_type{}, den_new, off_new)
                                          : weigh_row(std::false_type{}, den_new, off_new);
-                // a row that has seen nothing takes its first largest score as the reference
-                if (!__any_sync(0xffffffffu, unset ? most > -INFINITY : most > kRescaleAt)) break;
-                const float up = unset ? (most > -INFINITY ? most : 0.f) : fmaxf(most, 0.f);  // the reference moves up by this
+                // a row that has seen nothing takes its first largest score as the
+                // reference.  Past this barrier both halves have read their scores.
+                if (!pair_any(unset ? most > -INFINITY : most > kRescaleAt)) break;
+                largest[half * kTileRows + r] = most;
+                pair_sync();
+                const float m = fmaxf(most, largest[(half ^ 1) * kTileRows + r]);
+                const float up = unset ? (m > -INFINITY ? m : 0.f) : fmaxf(m, 0.f);  // the reference moves up by this
                 const float down = unset ? 1.f : exp2_approx(-up);
-                unset = unset && !(most > -INFINITY);
+                unset = unset && !(m > -INFINITY);
                 minus_ref -= up;
                 den = mul2(den, pair(down, down));
                 off = mul2(off, pair(down, down));
-                if (j > 0) {  // O, once the products so far are in it
-                    ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status);
+                if (j > 0) {  // O, once the products so far are in it: half of its columns each
+                    ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status) && ok;
                     tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
+                    for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
                         uint32_t o[32];
                         tmem_load32(mine + 128 + c, o);
                         tc_wait_ld();
@@ -254,8 +276,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             den = den_new;
             off = off_new;
             __syncwarp();
-            tmem_store32(mine + 64 * b, hi);
-            if constexpr (PRECISE) tmem_store32(mine + 64 * b + 32, lo);
+            tmem_store16(mine + 64 * b + 16 * half, hi);
+            if constexpr (PRECISE) tmem_store16(mine + 64 * b + 32 + 16 * half, lo);
             tc_wait_st();
             tc_fence_before();
             mbar_arrive(p_full + 8 * b);
@@ -265,12 +287,17 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             ok = phase_wait(kv_empty + 8 * ((steps - 1) & 1), (steps - 1) >> 1 & 1, p.status);
             tc_fence_after();
         }
-        const float2 d2 = unpair(den), o2 = unpair(off);
-        const float row_den = d2.x + d2.y, row_off = o2.x + o2.y;
+        {
+            const float2 d2 = unpair(den), o2 = unpair(off);
+            sums[half * kTileRows + r] = d2.x + d2.y;
+            sums[(2 + half) * kTileRows + r] = o2.x + o2.y;
+        }
+        pair_sync();
+        const float row_den = sums[r] + sums[kTileRows + r], row_off = sums[2 * kTileRows + r] + sums[3 * kTileRows + r];
         const float inv = it.slot >= 0 ? 1.f : row_den != 0.f ? __frcp_rn(row_den) : 0.f;
         float* part = it.slot >= 0 ? p.partials + ((int64_t)it.slot * p.kv_heads + hk) * kTileRows * (D + 2) : nullptr;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
             uint32_t o[32] = {};
             __syncwarp();
             if (steps > 0) {
@@ -290,12 +317,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 else store_channels<4>(p.o, out_row * D + g * (D / 8) + c / 8, v, p.o_dtype);
             }
         }
-        if (part && valid)
+        if (part && valid && half == 0)
             *reinterpret_cast<float2*>(part + kTileRows * D + 2 * r) = make_float2(unset ? kNoReference : -minus_ref, row_den);
         tc_fence_before();
-    } else if (warp < 8 && live) {
+    } else if (warp < kRowWarps + kCodeWarps && live) {
         // ------------------------------------------------------------ codes
-        const int dw = warp - 4, g = lane >> 2, t = lane & 3;
+        const int dw = warp - kRowWarps, g = lane >> 2, t = lane & 3;
         const int64_t page_bytes = (int64_t)p.kv_heads * RB;
         const int* list = p.tables + (int64_t)it.request * p.table_stride;
         const int last_seen = it.context + last_row / p.group;
@@ -361,7 +388,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             fence_proxy_async_shared();
             mbar_arrive(kv_full + 8 * b);
         }
-    } else if (warp == 8 && live && steps > 0) {
+    } else if (warp == kRowWarps + kCodeWarps && live && steps > 0) {
         // ------------------------------------------------------------ products
         ok = phase_wait(q_full, 0, p.status);
         auto weigh = [&](int j) {  // O += P V of step j
@@ -399,7 +426,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         if (ok) weigh(steps - 1);
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kRowWarps + kCodeWarps) {
         tc_fence_after();
         tmem_free(tmem, C::TMEM_COLUMNS);
     }

@@ -73,6 +73,12 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&v)[32
         F3S_W8(v, 8), F3S_W8(v, 16), F3S_W8(v, 24), "r"(at)
         : "memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::F3S_W8(v, 0),
+        F3S_W8(v, 8), "r"(at)
+        : "memory");
+}
 #undef F3S_R8
 #undef F3S_W8
 
