@@ -520,9 +520,7 @@ static int attend_variant(const AttendParams& p, int64_t units, cudaStream_t str
 
 template <int NT>
 static int attend_launch(const AttendParams& p, int head_dim, int64_t units, cudaStream_t stream) {
-    // fp32 results take the exact form of P; fp16 and bf16 ones round it to fp16,
-    // as much as an fp16 result is rounded
-    const bool precise = p.o_dtype == F3S_OUT_F32;
+    const bool precise = weights_in_full(p.o_dtype);
     if (head_dim == 64)
         return precise ? attend_variant<64, NT, true>(p, units, stream) : attend_variant<64, NT, false>(p, units, stream);
     return precise ? attend_variant<128, NT, true>(p, units, stream) : attend_variant<128, NT, false>(p, units, stream);

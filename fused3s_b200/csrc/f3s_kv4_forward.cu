@@ -787,9 +787,7 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
     F3S_CUDA_TRY(cudaMemsetAsync(base, 0, sizeof(f3s::WindowPieces), s));
     f3s::k_window_pieces<<<(unsigned)((num_items + 255) / 256), 256, 0, s>>>(w);
     F3S_LAUNCH_CHECK();
-    // fp32 results take the exact form of P; fp16 and bf16 ones round it to fp16,
-    // as much as an fp16 result is rounded
-    const bool precise = o_dtype == F3S_OUT_F32;
+    const bool precise = f3s::weights_in_full(o_dtype);
     const int st = head_dim == 64 ? (precise ? f3s::window_launch<64, true>(p, units, s) : f3s::window_launch<64, false>(p, units, s))
                                   : (precise ? f3s::window_launch<128, true>(p, units, s) : f3s::window_launch<128, false>(p, units, s));
     if (st != F3S_SUCCESS || L.splits_cap == 0 || w.piece == INT32_MAX) return st;  // no window is split

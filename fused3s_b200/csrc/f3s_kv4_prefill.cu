@@ -448,7 +448,7 @@ static int tiles_variant(const AttendParams& p, int64_t units, cudaStream_t stre
 }
 
 int attend_tiles128(const AttendParams& p, int head_dim, int64_t units, cudaStream_t stream) {
-    const bool precise = p.o_dtype == F3S_OUT_F32;
+    const bool precise = weights_in_full(p.o_dtype);
     if (head_dim == 64) return precise ? tiles_variant<64, true>(p, units, stream) : tiles_variant<64, false>(p, units, stream);
     return precise ? tiles_variant<128, true>(p, units, stream) : tiles_variant<128, false>(p, units, stream);
 }
