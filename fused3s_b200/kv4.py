@@ -23,7 +23,10 @@ then fused3s_forward_kv4(Q, cache, fmt, order=order).
 The byte layout of a page is described in include/fused3s.h.  Every call runs
 on the current stream of its tensors' device, allocates its outputs and
 scratch from torch's allocator on that stream (so it can be captured into a
-CUDA graph) and does not synchronise unless check_status is set.
+CUDA graph) and does not synchronise unless check_status is set.  Errors that
+a kernel finds in store_kv4, load_kv4 and fused3s_forward_kv4 are kept in one
+status word per device until a call with check_status raises them; those of
+build_block_tables and attention_kv4 in the block tables (status()).
 """
 from __future__ import annotations
 
@@ -34,7 +37,7 @@ import torch
 
 from . import _lib
 from ._lib import check
-from .api import _OUT_DTYPES, _WS, BlockSparseFormat, _default_device, generate_balanced_window_order
+from .api import _OUT_DTYPES, BlockSparseFormat, _default_device, generate_balanced_window_order
 
 PAGE_TOKENS = 16
 _RECORDS = {16 * d + 128: d for d in (64, 128)}
@@ -54,12 +57,29 @@ def _raw_stream(index: int) -> int:
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
+_STATUS = {}  # one status word per device for store, load and the graph forward
+
+
+def _status(device: torch.device) -> torch.Tensor:
+    """The device's status word: kernels only set it where it is 0, so all streams
+    and captured graphs share it.  Made before any capture, with the first cache."""
+    ws = _STATUS.get(device.index)
+    if ws is None:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("make the device's first KV4Cache before capturing a CUDA graph")
+            ws = torch.zeros(256, dtype=torch.uint8, device=device)
+            torch.cuda.current_stream(device).synchronize()
+        _STATUS[device.index] = ws
+    return ws
+
+
 class KV4Cache:
     """4-bit K / V of `num_pages` pages: pages uint8 [num_pages, kv_heads,
     16 * head_dim + 128], contiguous, on a CUDA device.  Wraps the tensor; a
     page of zeros holds zeros."""
 
-    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim", "device")
+    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim", "device", "status_ptr")
 
     def __init__(self, pages: torch.Tensor):
         if pages.dtype != torch.uint8 or pages.dim() != 3:
@@ -76,6 +96,7 @@ class KV4Cache:
         self.head_dim = _RECORDS[record]
         self.pages = pages
         self.device = pages.device
+        self.status_ptr = _status(self.device).data_ptr()
 
 
 def empty_kv4_cache(num_pages: int, kv_heads: int, head_dim: int, device=None) -> KV4Cache:
@@ -112,16 +133,6 @@ def _check_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, device: t
     return ptr, strides
 
 
-_ROWS_WS = {}  # status words of store, load and the graph forward, one per device and stream
-
-
-def _rows_workspace(index: int, stream: int) -> torch.Tensor:
-    ws = _ROWS_WS.get((index, stream))
-    if ws is None:
-        ws = _ROWS_WS[(index, stream)] = _WS.get(torch.device("cuda", index), "kv4", 256)
-    return ws
-
-
 def store_kv4(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, cache: KV4Cache,
               check_status: bool = False) -> KV4Cache:
     """Quantise row i of K and V (fp16 or bf16 [n, kv_heads, head_dim], strided
@@ -145,7 +156,7 @@ def store_kv4(K: torch.Tensor, V: torch.Tensor, slots: torch.Tensor, cache: KV4C
             return store_kv4(K, V, slots, cache, check_status)
     lib = _lib.load()
     stream = _raw_stream(device.index)
-    ws = _rows_workspace(device.index, stream).data_ptr()
+    ws = cache.status_ptr
     st = lib.f3s_kv4_store(k, v, _IN_DTYPES[K.dtype], ks[0], ks[1], vs[0], vs[1], slots.data_ptr(), n,
                            cache.pages.data_ptr(), cache.num_pages, cache.kv_heads, cache.head_dim, ws, 256, stream)
     if st:
@@ -172,7 +183,7 @@ def load_kv4(cache: KV4Cache, slots: torch.Tensor, dtype: torch.dtype = torch.fl
     v = torch.empty_like(k)
     lib = _lib.load()
     stream = _raw_stream(device.index)
-    ws = _rows_workspace(device.index, stream).data_ptr()
+    ws = cache.status_ptr
     st = lib.f3s_kv4_load(cache.pages.data_ptr(), cache.num_pages, cache.kv_heads, cache.head_dim, slots.data_ptr(), n,
                           k.data_ptr(), v.data_ptr(), _OUT_DTYPES[dtype], ws, 256, stream)
     if st:
@@ -396,7 +407,7 @@ def fused3s_forward_kv4(Q: torch.Tensor, cache: KV4Cache, fmt: BlockSparseFormat
     out = _result(Q, out, out_dtype, device)
     lib = _lib.load()
     stream = _raw_stream(device.index)
-    ws = _rows_workspace(device.index, stream).data_ptr()
+    ws = cache.status_ptr
     items, blocks = order.numel(), fmt.num_blocks
     size = lib.f3s_kv4_forward_scratch_size(items, blocks, heads, cache.kv_heads, head_dim)
     scratch = torch.empty(size, dtype=torch.uint8, device=device)

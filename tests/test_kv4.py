@@ -435,18 +435,24 @@ def test_attention_extreme_sizes(lib, size):
 
 
 @gpu
-def test_attention_leaves_out_what_is_masked(lib):
+@pytest.mark.parametrize("lengths,heads,d", [
+    ([(20, 3), (0, 5), (33, 1)], 4, 64),           # tiles of 8 query rows
+    ([(20, 13), (0, 5), (33, 11)], 4, 128),        # 32
+    ([(70, 90), (0, 130), (33, 60)], 4, 128),      # 128
+    ([(40, 41), (0, 50), (63, 70)], 12, 64)])      # 128, groups of 6
+def test_attention_leaves_out_what_is_masked(lib, lengths, heads, d):
     """NaN and garbage behind a request's end, in pages without an owner and behind
     table entries of -1; rows behind the last request stay as they were."""
-    lengths = [(20, 3), (0, 5), (33, 1)]
     tables, free, begin, num_pages = make_tables(lengths, 11)
-    cache = filled_cache(num_pages, 2, 64, 3)
-    bt = build(lengths, tables, free, begin, 12, heads=4, kv_heads=2)
+    cache = filled_cache(num_pages, 2, d, 3)
+    used = sum(n for _, n in lengths)
+    first = lengths[0][1]
+    bt = build(lengths, tables, free, begin, used + 3, heads=heads, kv_heads=2)
     rows = bt.tables.tolist()
-    q = randn((12, 4, 64), 4, torch.float16).cuda()
-    out = torch.full((12, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    q = randn((used + 3, heads, d), 4, torch.float16).cuda()
+    out = torch.full((used + 3, heads, d), 7.0, dtype=torch.float16, device="cuda")
     F.attention_kv4(q, cache, bt, scale=0.125, out=out, check_status=True)
-    assert (out[9:] == 7.0).all()
+    assert (out[used:] == 7.0).all()
     poisoned = F.KV4Cache(torch.full_like(cache.pages, 0xff))  # every scale and zero a NaN
     for (c, n), row in zip(lengths, rows):
         s = torch.tensor([row[p // 16] * 16 + p % 16 for p in range(c + n)], dtype=torch.int32, device="cuda")
@@ -455,21 +461,20 @@ def test_attention_leaves_out_what_is_masked(lib):
     # storing values that are 4-bit numbers already may move their scale by an fp16 step: compare with the cache's own
     again = torch.full_like(out, 7.0)
     F.attention_kv4(q, poisoned, bt, scale=0.125, out=again, check_status=True)
-    clean = F.KV4Cache(poisoned.pages.clone())
-    pk, pv = R.page_values(clean.pages, 64)
-    want, _, _ = want_attention(q[:9], clean, rows, lengths, 0.125, 4)
+    want, pk, pv = want_attention(q[:used], poisoned, rows, lengths, 0.125, heads)
     seen = pk[torch.isfinite(pk)], pv[torch.isfinite(pv)]
-    R.assert_close(again[:9], want, R.tolerance(q.double().cpu(), seen[0], seen[1], 0.125, want, torch.float16))
-    assert (again[9:] == 7.0).all()
-    # holes in a table: the first page of request 0, the only page of request 1
+    R.assert_close(again[:used], want, R.tolerance(q.double().cpu(), seen[0], seen[1], 0.125, want, torch.float16))
+    assert (again[used:] == 7.0).all()
+    # holes in a table: the first page of request 0, the first page of request 1
     holes = [list(r) for r in rows]
     holes[0][0] = -1
     holes[1][0] = -1
     bt.tables.copy_(i32(holes))
-    o = F.attention_kv4(q, cache, bt, scale=0.125, out_dtype=torch.float32, check_status=True)
-    want, pk, pv = want_attention(q[:9], cache, holes, lengths, 0.125, 4)
-    R.assert_close(o[:9], want, R.tolerance(q.double().cpu(), pk, pv, 0.125, want, torch.float32))
-    assert (o[3:8] == 0).all()
+    for dtype in (torch.float32, torch.bfloat16):
+        o = F.attention_kv4(q, cache, bt, scale=0.125, out_dtype=dtype, check_status=True)
+        want, pk, pv = want_attention(q[:used], cache, holes, lengths, 0.125, heads)
+        R.assert_close(o[:used], want, R.tolerance(q.double().cpu(), pk, pv, 0.125, want, dtype))
+        assert (o[first:first + min(5, lengths[1][1])] == 0).all()  # their only page is missing
     # a page outside the cache is left out too, and reported
     for bad in (num_pages, 2 ** 31 - 1, -2):
         holes[1][0] = bad
@@ -480,15 +485,64 @@ def test_attention_leaves_out_what_is_masked(lib):
 
 
 @gpu
-def test_attention_nan_reaches_only_who_sees_it(lib):
-    lengths = [(20, 4)]
+@pytest.mark.parametrize("heads,kv_heads,d,dtype,out_dtype", [
+    (4, 4, 64, torch.float16, torch.float16), (8, 1, 128, torch.bfloat16, torch.bfloat16),
+    (6, 2, 128, torch.float16, torch.float32), (14, 2, 64, torch.bfloat16, torch.float32)])
+@pytest.mark.parametrize("lengths", [
+    [(0, 300)], [(500, 129), (3, 200)], [(0, 97), (1, 300), (700, 16)], [(6000, 150)]])
+def test_attention_many_new_tokens(lib, lengths, heads, kv_heads, d, dtype, out_dtype):
+    """Tiles of 128 query rows: alone, ragged, behind contexts, cut into pieces."""
+    run_attention(lengths, heads, kv_heads, d, dtype, out_dtype, seed=6, pad=2)
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-4, 300.0])
+def test_attention_many_new_tokens_extreme_sizes(lib, size):
+    lengths = [(60, 200)]
+    tables, free, begin, num_pages = make_tables(lengths, 7)
+    cache = filled_cache(num_pages, 2, 64, 5, size)
+    q = randn((200, 4, 64), 8, torch.bfloat16, 1.0 / max(size, 1.0)).cuda()
+    # rows of very different sizes in one tile
+    q *= torch.exp2(torch.arange(200, device="cuda") % 23 - 11.0)[:, None, None].to(torch.bfloat16)
+    bt = build(lengths, tables, free, begin, 200, heads=4, kv_heads=2)
+    o = F.attention_kv4(q, cache, bt, scale=0.01, out_dtype=torch.float32)
+    want, pk, pv = want_attention(q, cache, bt.tables.tolist(), lengths, 0.01, 4)
+    R.assert_close(o, want, R.tolerance(q.double().cpu(), pk, pv, 0.01, want, torch.float32))
+    for _ in range(5):
+        assert torch.equal(F.attention_kv4(q, cache, bt, scale=0.01, out_dtype=torch.float32), o)
+
+
+@gpu
+def test_attention_rising_scores(lib):
+    """Scores that keep growing along the context: the reference moves again and again."""
+    for new, heads in ((1, 2), (11, 2), (150, 2)):
+        lengths = [(800, new)]
+        tables, free, begin, num_pages = make_tables(lengths, 3)
+        cache = F.empty_kv4_cache(num_pages, 1, 64)
+        bt = build(lengths, tables, free, begin, new, heads=heads, kv_heads=1)
+        row = bt.tables.tolist()[0]
+        n = 800 + new
+        slots = i32([row[p // 16] * 16 + p % 16 for p in range(n)])
+        k = torch.ones(n, 1, 64) * (torch.arange(n) / 100.0)[:, None, None]
+        v = randn((n, 1, 64), 2)
+        F.store_kv4(k.half().cuda(), v.half().cuda(), slots, cache)
+        q = torch.ones(new, heads, 64, dtype=torch.float16, device="cuda")
+        o = F.attention_kv4(q, cache, bt, scale=0.5, out_dtype=torch.float32)
+        want, pk, pv = want_attention(q, cache, [row], lengths, 0.5, heads)
+        R.assert_close(o, want, R.tolerance(q.double().cpu(), pk, pv, 0.5, want, torch.float32))
+
+
+@gpu
+@pytest.mark.parametrize("new", [4, 100])
+def test_attention_nan_reaches_only_who_sees_it(lib, new):
+    lengths = [(20, new)]
     tables, free, begin, num_pages = make_tables(lengths, 12)
     cache = filled_cache(num_pages, 1, 64, 3)
-    bt = build(lengths, tables, free, begin, 4, heads=2, kv_heads=1)
+    bt = build(lengths, tables, free, begin, new, heads=2, kv_heads=1)
     k, v = F.load_kv4(cache, bt.slots, torch.float16)
     v[2] = math.nan
     F.store_kv4(k, v, bt.slots, cache)
-    q = randn((4, 2, 64), 4, torch.float16).cuda()
+    q = randn((new, 2, 64), 4, torch.float16).cuda()
     o = F.attention_kv4(q, cache, bt, out_dtype=torch.float32)
     assert torch.isfinite(o[:2]).all() and torch.isnan(o[2:]).all()
     q[1, 1, 5] = math.nan
@@ -603,6 +657,44 @@ def test_graph_forward_many_units_empty_and_hub_windows(lib):
         F.fused3s_forward_kv4(q, cache, fmt, order=i32(order), out=out, scale=0.125, check_status=True)
         R.assert_close(out[64:80], want[64:80], R.tolerance(q.double().cpu(), seen[0], seen[1], 0.125, want[64:80], torch.float32))
         assert not out[:64].any() and not out[80:].any()
+
+
+@gpu
+def test_graph_forward_without_edges(lib):
+    fmt = F.convert_csr_to_block_sparse(50, np.zeros(51, dtype=np.int32), np.zeros(0, dtype=np.int32))
+    cache = filled_cache(4, 2, 64, 1)
+    q = randn((50, 2, 64), 5, torch.float16).cuda()
+    o = F.fused3s_forward_kv4(q, cache, fmt, check_status=True)
+    assert (o == 0).all()
+    fmt = F.convert_csr_to_block_sparse(0, np.zeros(1, dtype=np.int32), np.zeros(0, dtype=np.int32))
+    assert F.fused3s_forward_kv4(q[:0], cache, fmt).shape == (0, 2, 64)
+
+
+@gpu
+def test_graph_forward_captured_on_several_streams(lib):
+    """Two captured graphs and an eager call of the same forward at the same time."""
+    n, heads, d = 3000, 4, 64
+    _, fmt = graph_case(n, heads, d, 5, edges=20000)
+    cache = filled_cache(fmt.num_row_windows, heads, d, 4)
+    order = F.generate_balanced_window_order(fmt)
+    q = randn((n, heads, d), 5, torch.bfloat16).cuda()
+    want = F.fused3s_forward_kv4(q, cache, fmt, order=order, scale=0.125, out_dtype=torch.bfloat16)
+    outs = [torch.zeros_like(want) for _ in range(2)]
+    graphs = []
+    for out in outs:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            F.fused3s_forward_kv4(q, cache, fmt, order=order, scale=0.125, out=out)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        again = F.fused3s_forward_kv4(q, cache, fmt, order=order, scale=0.125, out_dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    assert torch.equal(again, want) and torch.equal(outs[0], want) and torch.equal(outs[1], want)
 
 
 @gpu
@@ -739,12 +831,13 @@ def test_captured_step_replays_with_new_lengths(lib):
 
 
 @gpu
-def test_calls_on_two_streams_share_tables_and_cache(lib):
-    lengths = [(700, 1), (90, 2), (0, 5)]
+@pytest.mark.parametrize("lengths", [[(700, 1), (90, 2), (0, 5)], [(700, 100), (0, 333)]])
+def test_calls_on_two_streams_share_tables_and_cache(lib, lengths):
     tables, free, begin, num_pages = make_tables(lengths, 21)
     cache = filled_cache(num_pages, 2, 128, 3)
-    bt = build(lengths, tables, free, begin, 8, heads=8, kv_heads=2)
-    qs = [randn((8, 8, 128), s, torch.bfloat16).cuda() for s in range(4)]
+    tokens = sum(n for _, n in lengths)
+    bt = build(lengths, tables, free, begin, tokens, heads=8, kv_heads=2)
+    qs = [randn((tokens, 8, 128), s, torch.bfloat16).cuda() for s in range(4)]
     want = [F.attention_kv4(q, cache, bt, scale=0.1) for q in qs]
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in qs]
