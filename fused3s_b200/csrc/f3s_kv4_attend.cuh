@@ -18,9 +18,27 @@ struct AttendParams {
     int* status;
     float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head
     const Kv4PlanHeader* plan;
+    int tile_rows, items_cap;
+    int num_requests, num_tokens;
     const int* tables;
     int64_t table_stride;
 };
+
+// True for a plan made with this call's sizes; any other's items would reach past
+// this call's arrays.
+__device__ __forceinline__ bool plan_fits(const AttendParams& p, const int4& counts, const int4& made_with) {
+    return counts.z == p.items_cap && counts.w == p.tile_rows && made_with.x == p.heads && made_with.y == p.kv_heads &&
+           made_with.z == p.num_requests && made_with.w == p.num_tokens;
+}
+
+// The plan's work items; 0, and F3S_ERR_BAD_FORMAT in its status, if it is not this call's.
+__device__ __forceinline__ int plan_items(const AttendParams& p) {
+    const int4* h = reinterpret_cast<const int4*>(&p.plan->num_items);
+    const int4 counts = h[0], made_with = h[1];
+    if (plan_fits(p, counts, made_with)) return counts.x;
+    if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
+    return 0;
+}
 
 // Tiles of 128 query rows on tcgen05 (f3s_kv4_prefill.cu); units: an upper bound.
 int attend_tiles128(const AttendParams& p, int head_dim, int64_t units, cudaStream_t stream);

@@ -17,6 +17,12 @@
 // and read as pairs; the arithmetic on scores runs on pairs of fp32 numbers.
 // tcgen05's M = 64 / 128 rows would stand mostly empty at 16 rows per window.
 //
+// Bound: instruction issue (56 % of the slots, mma.sync 43 %), since each window
+// unpacks its pages for itself.  131,057 nodes of 8 heads, D = 64, 22 blocks per window
+// (94 GFLOP, 508 MB from HBM, fp16 O): 632 us; the copies alone take 219 us.  40,009
+// nodes of 4 / 2 heads, D = 128, 80 blocks per window (105 GFLOP, 92 % of
+// the pages from L2, bf16 O): 455 us.
+//
 #include <algorithm>
 #include "f3s_kv4_math.cuh"
 
@@ -60,7 +66,8 @@ struct WindowParams {
 // Pieces of at most `piece` blocks: half of a thread block's even share of the
 // work (3 of them per SM; a quarter costs more in sums to add, all of it leaves a
 // tail: 470 + 9, 468 + 25 and 545 + 8 us for 40,009 nodes, d = 128), and 8 per warp
-// that takes them in any case.
+// that takes them in any case (2,708 nodes of one head: 24.7 us; with 4 per warp 30.8, with
+// 16 28.8).
 struct WindowPieceLayout {
     int piece;
     int64_t extra_cap, splits_cap, slots_cap;

@@ -12,12 +12,10 @@ namespace f3s {
 // tile, for every K/V head.
 struct Kv4PlanHeader {
     WsHeader ws;  // first: a plan is a workspace to f3s_workspace_status
-    int num_items;
-    int num_splits;
-    int items_cap, splits_cap;
-    int tile_rows, group, kv_heads, num_requests, num_tokens;
-    int max_parts;
-    int pad[54];
+    int num_items, num_splits;
+    int items_cap, tile_rows;
+    int heads, kv_heads, num_requests, num_tokens;  // what the plan was made with
+    int pad[56];
 };
 static_assert(sizeof(Kv4PlanHeader) == 512, "plan header is 512 bytes");
 

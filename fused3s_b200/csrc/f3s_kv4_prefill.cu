@@ -21,9 +21,10 @@
 // banks: row r holds channel (r % 8) * D / 8 + r / 8.
 //
 // Bound: the weights (13 instructions and 2.5 loads from shared memory per two
-// scores), then the products (128 x 64 x D twice per step).  One thread per row with
-// 64 tokens took 316 us where two take 255 us (prompts of 147 GFLOP;
-// mma.sync with 32 rows took 506).
+// scores; issue slots 39 % busy), then the products (128 x 64 x D twice per step;
+// tensor pipe 16 %).  Five prompts of up to 3,200 tokens, 32 / 8 heads, D = 128, 81
+// GFLOP: 255 us, 319 TFLOP/s.  With one thread per row and 64 tokens each 316 us;
+// mma.sync with 32 rows 506.
 #include <algorithm>
 #include <type_traits>
 #include "f3s_kv4_attend.cuh"
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
     launch_dependents();
     wait_for_primary();  // the plan
     const int item = blockIdx.x / p.kv_heads, hk = blockIdx.x - item * p.kv_heads;
-    const bool live = item < p.plan->num_items;
+    const bool live = item < plan_items(p);
     Kv4Item it{};
     if (live) {
         const int4* src = reinterpret_cast<const int4*>(reinterpret_cast<const Kv4Item*>(p.plan + 1) + item);

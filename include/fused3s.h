@@ -490,8 +490,10 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
  *            (multiples of 8; head_dim contiguous; 16-byte aligned)
  *   d_O      contiguous [num_tokens][heads][head_dim] of o_dtype; rows behind
  *            the last new token are not written
- *   d_tables, table_stride, num_requests, num_tokens, heads, kv_heads: those that the plan was made with; d_plan is not changed but for
- *            its status, so several calls may share it
+ *   d_tables, table_stride, num_requests, num_tokens, heads, kv_heads: those
+ *            that the plan was made with (a plan of other sizes is reported as
+ *            F3S_ERR_BAD_FORMAT in its status, and nothing is written); d_plan
+ *            is not changed but for its status, so several calls may share it
  *   d_scratch: f3s_kv4_attention_scratch_size bytes, 16-byte aligned, not
  *            shared by calls that may overlap; needs no initialisation
  * A table entry of -1 holds no tokens (they are left out); one outside the
@@ -515,8 +517,8 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
  * window lists and slabs as f3s_forward_ex.  num_pages >= ceil(num_nodes / 16).
  * num_blocks (the active blocks of the listed windows, or an estimate) sets how
  * heavy windows are cut into pieces for several SMs, merged in order, so no plan
- * is needed; it does not change which blocks are computed.  d_workspace (f3s_forward_workspace_size bytes, zeroed once)
- * keeps the status; d_scratch: f3s_kv4_forward_scratch_size bytes, 16-byte
+ * is needed; it does not change which blocks are computed.  d_workspace
+ * (f3s_forward_workspace_size bytes, zeroed once) keeps the status; d_scratch: f3s_kv4_forward_scratch_size bytes, 16-byte
  * aligned, not shared by calls that may overlap, needs no initialisation.
  * ---------------------------------------------------------------------- */
 size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t kv_heads,

@@ -566,6 +566,47 @@ def test_attention_strided_q_out_and_repeats(lib):
 
 
 @gpu
+@pytest.mark.parametrize("new", [1, 40, 100])
+def test_attention_refuses_another_plan(lib, new):
+    """A plan made for other sizes, an empty one and one of stray bytes write nothing and are reported."""
+    requests, tokens, d = 3, 3 * new, 64
+    made = dict(requests=requests, tokens=tokens, heads=8, kv_heads=4)
+    tables = torch.zeros(requests + 1, 8, dtype=torch.int32, device="cuda")
+    cache = F.empty_kv4_cache(32, 8, d)
+    cache.pages.zero_()
+    free = torch.arange(32, dtype=torch.int32, device="cuda")
+    Q = torch.zeros(tokens + 1, 16, d, dtype=torch.float16, device="cuda")
+
+    def call(bt, requests, tokens, heads, kv_heads):
+        out = torch.full((tokens, heads, d), 7.0, device="cuda")
+        size = lib.f3s_kv4_attention_scratch_size(requests, tokens, heads, kv_heads, d)
+        scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+        st = lib.f3s_kv4_attention(Q.data_ptr(), 1, heads * d, d, cache.pages.data_ptr(), 32 * 8 // kv_heads,
+                                   tables.data_ptr(), tables.stride(0), bt.buffer.data_ptr(), requests, tokens, heads,
+                                   kv_heads, d, 1.0, out.data_ptr(), 0, scratch.data_ptr(), size,
+                                   torch.cuda.current_stream().cuda_stream)
+        assert st == _lib.F3S_SUCCESS
+        torch.cuda.synchronize()
+        return out, bt.status()
+
+    def build():
+        return F.build_block_tables(i32([0] * requests), i32([new] * requests), tables[:requests], free, None, tokens,
+                                    heads=8, kv_heads=4)
+
+    out, status = call(build(), **made)
+    assert status == _lib.F3S_SUCCESS and (out != 7).all()
+    for other in (dict(heads=4), dict(heads=16, kv_heads=8), dict(kv_heads=8), dict(requests=requests + 1),
+                  dict(requests=requests - 1), dict(tokens=tokens + 1), dict(tokens=tokens - 1)):
+        out, status = call(build(), **{**made, **other})
+        assert status == _lib.F3S_ERR_BAD_FORMAT and (out == 7).all()
+    for byte in (0, 0x7f):
+        bt = build()
+        bt.buffer[64 : bt.plan_bytes // 4] = byte * 0x01010101  # all but the status
+        out, status = call(bt, **made)
+        assert status == _lib.F3S_ERR_BAD_FORMAT and (out == 7).all()
+
+
+@gpu
 def test_attention_offsets_beyond_32_bits(lib):
     """A cache of more than 2^32 bytes: pages at its end."""
     d, kv_heads = 128, 8
