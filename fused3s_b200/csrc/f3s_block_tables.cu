@@ -180,7 +180,9 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
         for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
         if ((tid & 31) == 0 && work) atomicAdd(&s_work, work);
         __syncthreads();
-        piece = (int)min(max((s_work + p.target - 1) / p.target, (unsigned long long)kKv4MinPiecePages), 1ull << 28);
+        const unsigned long long share = (s_work + p.target - 1) / p.target;
+        piece = (int)min(max(share, min(2 * share, (unsigned long long)kKv4LongPiecePages)), 1ull << 28);
+        piece = max(piece, kKv4MinPiecePages);
     }
 
     first_base = 0;
@@ -199,7 +201,7 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
         }
         BtRequest q = bt_request(p, c, n, first);
         if (r >= p.requests) q = BtRequest{};
-        const int parts = q.tiles ? (q.pages + piece - 1) / piece : 0;
+        const int parts = q.tiles ? kv4_parts(q.pages, piece) : 0;
         // new pages, items, and tiles cut in several (their slots are parts times as many)
         uint32_t v[3] = {(uint32_t)(q.pages - q.old_pages), min((uint32_t)q.tiles * (uint32_t)parts, kBtMost),
                          parts > 1 ? (uint32_t)q.tiles : 0u};
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
             for (uint32_t it = item_base + other_at; it < min(item_end, (uint32_t)p.items_cap); it += other_step) {
                 const int i = bt_find(s_item, here, it);
                 const BtRequest& w = s_req[i];
-                const int m = (w.pages + piece - 1) / piece;
+                const int m = kv4_parts(w.pages, piece);
                 const int local = (int)(it - s_item[i]);
                 const int nth = local / m, part = local - nth * m;
                 // a request's last rows see the most: their tiles begin first

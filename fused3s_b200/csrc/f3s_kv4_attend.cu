@@ -11,7 +11,7 @@
 // S^T = K Q^T and O^T = V^T P^T run on mma.m16n8k16 with the cache as the 16-row
 // operand (unpacked in registers, one AND per two values, f3s_kv4.cuh) and 8 NT
 // query rows as columns; P goes from accumulator to operand layout through
-// movmatrix.  tcgen05's M = 64 / 128 rows would stand mostly empty: 4 to 32 query
+// movmatrix.  tcgen05's M = 64 / 128 rows would stand mostly empty: 4 to 16 query
 // rows share a page.
 //
 // Bound: HBM and instruction issue together.  64 requests of up to 8,191 tokens, one
@@ -28,19 +28,17 @@ constexpr int kAttendWarps = 4;
 template <int D, int NT>
 struct AttendCfg {
     static constexpr int RB = kv4_record_bytes(D);
-    static constexpr int PP = NT == 4 ? 1 : 2;  // pages per step and stage
+    static constexpr int PP = 2;  // pages per step and stage
     static constexpr int STAGES = (D == 64 ? 8 : 4) / PP;
     static constexpr int STAGE_BYTES = PP * RB;
     static constexpr int RING = kAttendWarps * STAGES * STAGE_BYTES;
-    static constexpr bool Q_SMEM = NT == 4;  // four warps per unit only: they share it
-    static constexpr int Q_BYTES = Q_SMEM ? 8 * NT * D * 2 : 0;
     static constexpr int OPITCH = D + 4;
     static constexpr int MERGE = kAttendWarps * 8 * NT * (OPITCH + 2) * 4;
-    static constexpr int DATA = RING + Q_BYTES > MERGE ? RING + Q_BYTES : (MERGE + 127) / 128 * 128;
+    static constexpr int DATA = RING > MERGE ? RING : (MERGE + 127) / 128 * 128;
     static constexpr int BARS = DATA;
     static constexpr int SINK = BARS + kAttendWarps * STAGES * 8;  // one word per warp, written, never read
     static constexpr int SMEM = SINK + kAttendWarps * 4;
-    static constexpr int MIN_CTAS = NT == 4 ? 2 : NT == 2 && D == 128 ? 3 : 4;
+    static constexpr int MIN_CTAS = NT == 2 && D == 128 ? 3 : 4;
 };
 
 // PRECISE adds the part of P that rounding to fp16 drops with a second product,
@@ -135,10 +133,9 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     // ---- Q: rows g of each n-tile, channels t * D / 4 ..., as fp16 times a
     // power of two that brings the tile's largest to [2^9, 2^10); channels
     // whose codes come in units of 2^-24 another 2^4
-    uint32_t qf[C::Q_SMEM ? 1 : NT][C::Q_SMEM ? 1 : W][4];
+    uint32_t qf[NT][W][4];
     float qs[NT][2];  // sum of q (in the scores' unit) of rows 2t, 2t + 1
     float unit_scale;
-    uint4* qsm = reinterpret_cast<uint4*>(smem + C::RING);
     {
         float amax = 0.f;
         uint4 raw[NT][W];
@@ -205,12 +202,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                     const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[n]));
                     sum += (x.x + x.y) * (n & 1 ? 1.f : 0.0625f);
                 }
-                if constexpr (C::Q_SMEM) {
-                    if (warp == nt) qsm[(nt * W + w) * 32 + lane] = make_uint4(h[0], h[1], h[2], h[3]);
-                } else {
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) qf[nt][w][n] = h[n];
-                }
+                for (int n = 0; n < 4; ++n) qf[nt][w][n] = h[n];
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
@@ -221,7 +214,6 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             qs[nt][0] = __shfl_sync(0xffffffffu, sums[nt], 8 * t);      // row 2t is summed in lanes 4 * 2t ...
             qs[nt][1] = __shfl_sync(0xffffffffu, sums[nt], 8 * t + 4);  // row 2t + 1
         }
-        if constexpr (C::Q_SMEM) __syncthreads();
     }
 
     float acc[NT][D / 16][4];
@@ -269,17 +261,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                 const uint32_t a1[4] = {a8 & kNib0, b8 & kNib0, a8 & kNib1, b8 & kNib1};
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    uint32_t b[4];
-                    if constexpr (C::Q_SMEM) {
-                        const uint4 y = qsm[(nt * W + w) * 32 + lane];
-                        b[0] = y.x;
-                        b[1] = y.y;
-                        b[2] = y.z;
-                        b[3] = y.w;
-                    } else {
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) b[m] = qf[nt][w][m];
-                    }
+                    const uint32_t(&b)[4] = qf[nt][w];
                     if (w == 0) mma_16816_zero(s[nt], a0, b[0], b[1]);
                     else mma_16816(s[nt], a0, b[0], b[1]);
                     mma_16816(s[nt], a1, b[2], b[3]);
@@ -309,7 +291,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         // ---- masks: only where a page has tokens that some row must not see
         const int tok0 = (it.page0 + warp * PP + i * PP * kAttendWarps) * 16;
         if ((i * PP & 31) == 0) flags_now = flags;  // no later batch has been issued yet
-        if (tok0 + 16 * PP > open || (flags_now >> (i * PP & 31) & (PP == 2 ? 3u : 1u))) {
+        if (tok0 + 16 * PP > open || (flags_now >> (i * PP & 31) & 3u)) {
             __syncwarp();
 #pragma unroll
             for (int k = 0; k < PP; ++k) {
@@ -494,11 +476,13 @@ __global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p) {
     wait_for_primary();  // the sums
     const int4* h = reinterpret_cast<const int4*>(&p.plan->num_items);
     const int4 counts = h[0], made_with = h[1];
-    const int num_splits = plan_fits(p, counts, made_with) ? counts.y : 0;
+    const bool fits = plan_fits(p, counts, made_with);
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
+    const int num_splits = fits ? counts.y : 0;
     const int tq = p.tile_rows, group = p.group;
     const Kv4Split* splits =
         reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(p.plan + 1) + (int64_t)p.items_cap * sizeof(Kv4Item));
-    merge_rows<D>(num_splits, p.kv_heads, tq, min(tq, group), p.partials, p.o, p.o_dtype,
+    merge_rows<D>(num_splits, p.kv_heads, tq, p.live_rows, p.partials, p.o, p.o_dtype,
                   [&](int split, int hk, int r, int& slot, int& parts) -> int64_t {
                       const Kv4Split s = splits[split];
                       const int row = s.row0 + r, tok = row / group;
@@ -582,6 +566,7 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     p.partials = static_cast<float*>(d_scratch);
     p.tile_rows = L.tile_rows;
     p.items_cap = (int)L.items_cap;
+    p.live_rows = (int)std::min<int64_t>(L.tile_rows, (num_tokens * p.group + num_requests - 1) / num_requests);
     p.num_requests = num_requests;
     p.num_tokens = (int)num_tokens;
     p.tables = d_tables;
@@ -591,7 +576,6 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     int st;
     if (L.tile_rows == 8) st = f3s::attend_launch<1>(p, head_dim, units, s);
     else if (L.tile_rows == 16) st = f3s::attend_launch<2>(p, head_dim, units, s);
-    else if (L.tile_rows == 32) st = f3s::attend_launch<4>(p, head_dim, units, s);
     else st = f3s::attend_tiles128(p, head_dim, units, s);
     if (st != F3S_SUCCESS) return st;
     const int64_t blocks = std::min<int64_t>((int64_t)L.splits_cap * kv_heads * L.tile_rows,

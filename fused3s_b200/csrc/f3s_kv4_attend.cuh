@@ -19,6 +19,7 @@ struct AttendParams {
     float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head
     const Kv4PlanHeader* plan;
     int tile_rows, items_cap;
+    int live_rows;  // of a tile, on average
     int num_requests, num_tokens;
     const int* tables;
     int64_t table_stride;
@@ -31,13 +32,11 @@ __device__ __forceinline__ bool plan_fits(const AttendParams& p, const int4& cou
            made_with.z == p.num_requests && made_with.w == p.num_tokens;
 }
 
-// The plan's work items; 0, and F3S_ERR_BAD_FORMAT in its status, if it is not this call's.
+// The plan's work items; 0 if it is not this call's (which the merge reports).
 __device__ __forceinline__ int plan_items(const AttendParams& p) {
     const int4* h = reinterpret_cast<const int4*>(&p.plan->num_items);
     const int4 counts = h[0], made_with = h[1];
-    if (plan_fits(p, counts, made_with)) return counts.x;
-    if (blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
-    return 0;
+    return plan_fits(p, counts, made_with) ? counts.x : 0;
 }
 
 // Tiles of 128 query rows on tcgen05 (f3s_kv4_prefill.cu); units: an upper bound.

@@ -194,7 +194,8 @@ __device__ __forceinline__ void merge_rows(int count, int subs, int tq, int live
             float x[AHEAD][E];
 #pragma unroll
             for (int a = 0; a < AHEAD; ++a) {
-                const int64_t at = (int64_t)min(k + a * dk, parts - 1) * stride;
+                if (k + a * dk >= parts) break;
+                const int64_t at = (int64_t)(k + a * dk) * stride;
                 m[a] = ml[at / 2];
                 if constexpr (E == 4) {
                     const float4 y = *reinterpret_cast<const float4*>(src + at);

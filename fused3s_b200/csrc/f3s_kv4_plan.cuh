@@ -7,7 +7,7 @@
 namespace f3s {
 
 // Query rows of one request and one K/V head are numbered row = token * group
-// + head within the group; a tile is tile_rows of them (8, 16, 32 or 128), a piece
+// + head within the group; a tile is tile_rows of them (8, 16 or 128), a piece
 // a run of the pages that the tile sees.  A work item is one piece of one
 // tile, for every K/V head.
 struct Kv4PlanHeader {
@@ -38,8 +38,23 @@ struct Kv4Split {
 };
 static_assert(sizeof(Kv4Split) == 32, "two 16-byte loads");
 
-// A piece holds at least this many pages of a tile that is split.
-constexpr int kKv4MinPiecePages = 8;
+// A piece is share = W / target pages (W and target: kv4_plan_layout), two shares as
+// long as those are at most kKv4LongPiecePages, and kKv4MinPiecePages in any case.  A
+// block costs some 30 pages' time to begin and end, so shorter pieces lose more than
+// an even load gains.  Attention and merge, 32 / 8 heads, D = 128, one new token:
+//   64 requests of 65 pages      20.9 us with 64 (one piece each), 34.7 with 40 (two)
+//   4 requests of 1,000 pages    20.3 us with 64, 23.9 with 40
+//   64 of up to 512 pages        90.8 us with one share (with tables), 94.0 with two
+//   4 requests of 250 pages      11.6 us with 16 at least, 14.6 with 8
+//   1 request of 63 pages        8.0 us with 16 at least, 7.4 with 8
+constexpr int kKv4MinPiecePages = 16;
+constexpr int kKv4LongPiecePages = 64;
+
+// Pieces of a tile that sees so many pages: the nearest number, since a tile a little
+// longer than a piece costs less whole than in two; all that fit at the least size.
+__device__ __forceinline__ int kv4_parts(int pages, int piece) {
+    return max((pages + (piece == kKv4MinPiecePages ? piece - 1 : piece / 2)) / piece, 1);
+}
 
 struct Kv4PlanLayout {
     int tile_rows;
@@ -51,13 +66,23 @@ struct Kv4PlanLayout {
 // What a host can know before the lengths are read; num_tokens bounds the new
 // tokens.  With W = sum over tiles of the pages they see and pieces of
 // P >= W / target pages, the tiles have at most tiles + W / P pieces; those of
-// tiles cut in two or more hold more than P / 2 pages each.
+// tiles cut in two or more hold more than P / 2 pages each.  (A share is W / target.)
 inline Kv4PlanLayout kv4_plan_layout(int num_requests, int64_t num_tokens, int heads, int kv_heads, int sms) {
     Kv4PlanLayout L{};
     const int64_t group = heads / kv_heads;
     const int64_t rows = num_tokens * group;
     const int64_t mean = num_requests > 0 ? (rows + num_requests - 1) / num_requests : 0;
-    L.tile_rows = mean <= 8 ? 8 : mean <= 16 ? 16 : mean <= 96 ? 32 : 128;
+    // Rows per request -> us with tiles of 8, 16, 128 rows (64 requests of 1,024 tokens,
+    // 8 K/V heads, D = 128; 64 requests, 2 K/V heads, D = 64; 8 requests, 8 heads, D = 128):
+    //   24:  51, 55, 103
+    //   32:                16, 27, 47    21, 25, 48
+    //   48:  92, 79, 107
+    //   64: 120, 99, 108   26, 21, 37    21, 35, 56
+    //   96: 176, 143, 115  37, 31, 39
+    //  128: 232, 189, 123  46, 35, 41    34, 35, 56
+    //  256:                86, 65, 44    63, 54, 55
+    // Tiles of 32 rows on mma.sync were never faster than the best of these.
+    L.tile_rows = mean <= 32 ? 8 : mean <= 96 ? 16 : 128;
     const int64_t tiles = rows / L.tile_rows + num_requests;
     // twice as many pieces as blocks run at a time (4 per SM, 2 of 128 rows, one K/V head each),
     // so that blocks of unequal work even out
