@@ -472,17 +472,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 
 // The sums of split tiles: see merge_rows.
 template <int D>
-__global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p) {
+__global__ void __launch_bounds__(128) k_attend4_merge(const AttendParams p, const int tq, const int live) {
     wait_for_primary();  // the sums
     const int4* h = reinterpret_cast<const int4*>(&p.plan->num_items);
     const int4 counts = h[0], made_with = h[1];
     const bool fits = plan_fits(p, counts, made_with);
     if (!fits && blockIdx.x == 0 && threadIdx.x == 0) atomicCAS(p.status, 0, F3S_ERR_BAD_FORMAT);
     const int num_splits = fits ? counts.y : 0;
-    const int tq = p.tile_rows, group = p.group;
+    const int group = p.group;
     const Kv4Split* splits =
         reinterpret_cast<const Kv4Split*>(reinterpret_cast<const char*>(p.plan + 1) + (int64_t)p.items_cap * sizeof(Kv4Item));
-    merge_rows<D>(num_splits, p.kv_heads, tq, p.live_rows, p.partials, p.o, p.o_dtype,
+    merge_rows<D>(num_splits, p.kv_heads, tq, live, p.partials, p.o, p.o_dtype,
                   [&](int split, int hk, int r, int& slot, int& parts) -> int64_t {
                       const Kv4Split s = splits[split];
                       const int row = s.row0 + r, tok = row / group;
@@ -564,9 +564,7 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     p.plan = static_cast<const f3s::Kv4PlanHeader*>(d_plan);
     p.status = &static_cast<f3s::WsHeader*>(d_plan)->status;
     p.partials = static_cast<float*>(d_scratch);
-    p.tile_rows = L.tile_rows;
     p.items_cap = (int)L.items_cap;
-    p.live_rows = (int)std::min<int64_t>(L.tile_rows, (num_tokens * p.group + num_requests - 1) / num_requests);
     p.num_requests = num_requests;
     p.num_tokens = (int)num_tokens;
     p.tables = d_tables;
@@ -578,9 +576,12 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     else if (L.tile_rows == 16) st = f3s::attend_launch<2>(p, head_dim, units, s);
     else st = f3s::attend_tiles128(p, head_dim, units, s);
     if (st != F3S_SUCCESS) return st;
+    // rows of a tile, on average
+    const int live = (int)std::min<int64_t>(L.tile_rows, (num_tokens * p.group + num_requests - 1) / num_requests);
     const int64_t blocks = std::min<int64_t>((int64_t)L.splits_cap * kv_heads * L.tile_rows,
                                              8ll * f3s::num_sms_of_current_device());
-    return f3s::launch_after(head_dim == 64 ? f3s::k_attend4_merge<64> : f3s::k_attend4_merge<128>, (unsigned)blocks, 128, 0, s, p);
+    return f3s::launch_after(head_dim == 64 ? f3s::k_attend4_merge<64> : f3s::k_attend4_merge<128>, (unsigned)blocks, 128, 0, s, p,
+                             L.tile_rows, live);
 }
 
 }  // extern "C"

@@ -5,22 +5,24 @@
 
 namespace f3s {
 
+// No field more than fits: with 24 bytes of parameters more, the kernel of 128-row
+// tiles got other registers and took 271 us instead of 255.
 struct AttendParams {
     const void* q;
     int64_t q_token, q_head;  // strides in elements
     int q_bf16;
+    int items_cap;
     const uint8_t* pages;
     int num_pages;
     int kv_heads, heads, group;
     float scale;   // times log2(e)
+    int num_requests;
     void* o;       // contiguous [rows, heads, D] of o_dtype
     int o_dtype;
+    int num_tokens;
     int* status;
     float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head
     const Kv4PlanHeader* plan;
-    int tile_rows, items_cap;
-    int live_rows;  // of a tile, on average
-    int num_requests, num_tokens;
     const int* tables;
     int64_t table_stride;
 };
@@ -28,7 +30,7 @@ struct AttendParams {
 // True for a plan made with this call's sizes; any other's items would reach past
 // this call's arrays.
 __device__ __forceinline__ bool plan_fits(const AttendParams& p, const int4& counts, const int4& made_with) {
-    return counts.z == p.items_cap && counts.w == p.tile_rows && made_with.x == p.heads && made_with.y == p.kv_heads &&
+    return counts.z == p.items_cap && made_with.x == p.heads && made_with.y == p.kv_heads &&
            made_with.z == p.num_requests && made_with.w == p.num_tokens;
 }
 
