@@ -66,14 +66,17 @@ struct WindowParams {
 // Pieces of at most `piece` blocks: half of a thread block's even share of the
 // work (3 of them per SM; a quarter costs more in sums to add, all of it leaves a
 // tail: 470 + 9, 468 + 25 and 545 + 8 us for 40,009 nodes, d = 128), and 8 per warp
-// that takes them in any case (2,708 nodes of one head: 24.7 us; with 4 per warp 30.8, with
-// 16 28.8).
+// that takes them in any case (2,708 nodes of one head, as measured then: 24.7 us; with 4 per
+// warp 30.8, with 16 28.8).
 struct WindowPieceLayout {
     int piece;
     int64_t extra_cap, splits_cap, slots_cap;
     size_t items, splits, partials, total;
 };
 
+// Query heads to a block: 4, 2 or 1, as the counts divide.  With at most 1, 2 and 4 of
+// 8 heads 1,075, 800 and 632 us (131,057 nodes, d = 64), of 4 / 2 heads 599, 533 and 455 (40,009
+// nodes, d = 128); 2,708 nodes of 8 heads, d = 64, 56, 51 and 60.
 static int window_head_group(int heads, int group) {
     for (int hg = 4; hg > 1; hg >>= 1)
         if (heads % hg == 0 && (group % hg == 0 || hg % group == 0)) return hg;
