@@ -187,7 +187,9 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES) + 32 * half;
             const int tok0 = (it.page0 + 4 * j) * 16 + 32 * half;
             uint32_t hi[16], lo[PRECISE ? 16 : 1];  // P, two tokens each, and what its rounding drops
-            // Weights and sums against the reference as it stands; the largest score over it
+            // Weights and sums against the reference as it stands; the largest score.  A score
+            // is rounded before the reference is taken off, so that no weight passes
+            // 1 once the reference is the largest score, however large that is.
             auto weigh_row = [&](auto hides, uint64_t& den_out, uint64_t& off_out) {
                 constexpr bool HIDES = decltype(hides)::value;
                 float most = -INFINITY;
@@ -203,11 +205,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                     const ulonglong2 l = reinterpret_cast<const ulonglong2*>(tokens + 128)[c];
                     ulonglong2 ri = reinterpret_cast<const ulonglong2*>(tokens + 192)[c];
                     ulonglong2 y = reinterpret_cast<const ulonglong2*>(tokens + 256)[c];
-                    // scale s (q . u - z sum(q)) + log2 r - R
+                    // scale s (q . u - z sum(q)) + log2 r
                     uint64_t x[2] = {pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])),
                                      pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]))};
-                    x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), add2(l.x, mref2));
-                    x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), add2(l.y, mref2));
+                    x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), l.x);
+                    x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), l.y);
                     if constexpr (HIDES) {
                         // a hidden token's scale and zero may be anything, NaN too
                         const int left = limit - (tok0 + 4 * c);  // tokens up to this one are seen
@@ -224,14 +226,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                     }
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const float2 v = unpair(x[i]);
+                        const float2 v = unpair(x[i]), w = unpair(add2(x[i], mref2));
                         most = fmaxf(most, fmaxf(v.x, v.y));
-                        const float2 a = make_float2(exp2_approx(v.x), exp2_approx(v.y));
+                        const float2 a = make_float2(exp2_approx(w.x), exp2_approx(w.y));
                         const uint64_t a2 = pair(a.x, a.y);
                         hi[2 * c + i] = pack_half2(a.x, a.y);
                         if constexpr (PRECISE) {
-                            const float2 w = half2_floats(hi[2 * c + i]);
-                            lo[2 * c + i] = pack_half2(a.x - w.x, a.y - w.y);
+                            const float2 h = half2_floats(hi[2 * c + i]);
+                            lo[2 * c + i] = pack_half2(a.x - h.x, a.y - h.y);
                         }
                         d = fma2(a2, i ? ri.y : ri.x, d);
                         o = fma2(a2, i ? y.y : y.x, o);
@@ -244,19 +246,24 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             // the warp's first row sees the least
             const bool hides = tok0 + 32 > it.context + (it.row0 + 32 * quad) / p.group + 1;
             uint64_t den_new, off_new;
-            for (;;) {
+#pragma unroll 1
+            for (bool again = false;; again = true) {  // twice at most
                 const float most = hides ? weigh_row(std::true_type{}, den_new, off_new)
                                          : weigh_row(std::false_type{}, den_new, off_new);
-                // a row that has seen nothing takes its first largest score as the
-                // reference.  Past this barrier both halves have read their scores.
-                if (!pair_any(unset ? most > -INFINITY : most > kRescaleAt)) break;
+                // Past these barriers both halves have read their scores.
+                if (again) {
+                    pair_sync();
+                    break;
+                }
+                // a row that has seen nothing takes its first largest score as the reference
+                if (!pair_any(unset ? most > -INFINITY : most + minus_ref > kRescaleAt)) break;
                 largest[half * kTileRows + r] = most;
                 pair_sync();
                 const float m = fmaxf(most, largest[(half ^ 1) * kTileRows + r]);
-                const float up = unset ? (m > -INFINITY ? m : 0.f) : fmaxf(m, 0.f);  // the reference moves up by this
-                const float down = unset ? 1.f : exp2_approx(-up);
+                const float before = minus_ref;
+                if (m > -INFINITY) minus_ref = unset ? -m : fminf(minus_ref, -m);
+                const float down = unset ? 1.f : exp2_approx(minus_ref - before);
                 unset = unset && !(m > -INFINITY);
-                minus_ref -= up;
                 den = mul2(den, pair(down, down));
                 off = mul2(off, pair(down, down));
                 if (j > 0) {  // O, once the products so far are in it: half of its columns each
