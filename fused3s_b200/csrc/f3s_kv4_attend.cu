@@ -237,8 +237,11 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         const uint32_t st = i % STAGES, parity = i / STAGES & 1;
         bool ready = mbar_try_wait(bars + 8 * st, parity);
         if (!__all_sync(0xffffffffu, ready)) {
-            ready = phase_wait_slow(bars + 8 * st, parity, p.status);
-            if (!__all_sync(0xffffffffu, ready)) break;  // a wait ran out
+            ready = phase_wait_slow(bars + 8 * st, parity, p.status, p.status);
+            if (!__all_sync(0xffffffffu, ready)) {  // the wait ran out
+                ring_drain(bars, STAGES, i, min(i + STAGES, steps));
+                break;
+            }
         }
         uint32_t dep = 0;
         float x[PP][NT][4];

@@ -36,7 +36,8 @@ constexpr int kAttendThreads = (kConsumers + 1) * 32;
 // listed ones.
 struct WindowPieces {
     int extra, splits, slots, ticket;
-    int pad[60];
+    int stop;  // F3S_ERR_TIMEOUT once a wait of this launch ran out
+    int pad[59];
 };
 static_assert(sizeof(WindowPieces) == 256, "piece header is 256 bytes");
 
@@ -197,6 +198,16 @@ struct Unit {  // as the producer hands it to the consumers
 };
 
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
+// True if x is, in every consumer.
+__device__ __forceinline__ bool consumers_all(bool x) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred a, b;\n\tsetp.ne.u32 a, %1, 0;\n\tbar.red.and.pred b, 1, %2, a;\n\tselp.u32 %0, 1, 0, b;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)x), "n"(kConsumers * 32)
+        : "memory");
+    return all != 0;
+}
 
 // The producer warp: units, their block lists, the copies.
 template <int D>
@@ -208,7 +219,9 @@ __device__ __forceinline__ void window_produce(const WindowParams& p, uint32_t r
     const int stages = p.stages, stage_bytes = PP * p.kvs * RB, copy_bytes = p.kvs * RB;
     const int64_t page_bytes = (int64_t)p.kv_heads * RB;
     const int extra = min(p.pieces->extra, p.extra_cap);
+    int* stop = &p.pieces->stop;
     uint32_t n = 0;  // steps issued
+    auto end = [&] { ring_drain(full, stages, n > (uint32_t)stages ? n - stages : 0, n); };
     int ticket = 0;
     if (lane == 0) ticket = atomicAdd(&p.pieces->ticket, 1);
     for (int k = 0;; ++k) {
@@ -224,12 +237,12 @@ __device__ __forceinline__ void window_produce(const WindowParams& p, uint32_t r
         }
         const int count = piece.x >= 0 ? piece.z - piece.y : 0;
         const int* list = p.cols + piece.y;
-        if (!phase_wait(unit_empty + 8 * (k & 1), (k >> 1 & 1) ^ 1, p.status)) return;
+        if (!phase_wait(unit_empty + 8 * (k & 1), (k >> 1 & 1) ^ 1, p.status, stop)) return end();
         if (lane == 0) {
             unit_out[k & 1] = Unit{live, piece.x, piece.w, (count + PP - 1) / PP, head0};
             mbar_arrive(unit_full + 8 * (k & 1));
         }
-        if (!live) return;
+        if (!live) return end();
         if (piece.x >= 0) {  // the unit's Q rows, a line or more each, on their way to L2
             const int64_t row = (int64_t)(piece.x - p.q_window_base) * 16 + (lane & 15);
             if (row < p.q_rows) {
@@ -262,7 +275,7 @@ __device__ __forceinline__ void window_produce(const WindowParams& p, uint32_t r
             const uint32_t skip = __ballot_sync(0xffffffffu, mine && (!have || id < 0));
             const uint32_t tail = __ballot_sync(0xffffffffu, have && id == p.windows - 1);
             const uint32_t st = n & (stages - 1);
-            if (!phase_wait(empty + 8 * st, (n / stages & 1) ^ 1, p.status)) return;
+            if (!phase_wait(empty + 8 * st, (n / stages & 1) ^ 1, p.status, stop)) return end();
             if (lane == 0) {
                 flags_out[st] = (int)(skip | tail << 8);
                 mbar_arrive_expect_tx(full + 8 * st, min(PP, count - i) * copy_bytes);
@@ -324,11 +337,14 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
     float* tokens = reinterpret_cast<float*>(smem + C::TOKENS + warp * C::TOKEN_BYTES);
     uint4* qsm = reinterpret_cast<uint4*>(smem + C::Q + warp * C::Q_BYTES);
     const int page_stride = p.kvs * RB, stage_bytes = PP * page_stride;
+    int* stop = &p.pieces->stop;
     bool dead = false;  // a wait ran out: nothing more is read
     uint32_t done = 0;  // steps of the units before this one
 
     for (int k = 0;; ++k) {
-        if (!phase_wait(unit_full + 8 * (k & 1), k >> 1 & 1, p.status)) break;
+        bool ready = phase_wait(unit_full + 8 * (k & 1), k >> 1 & 1, p.status, stop);
+        if (turns > 1) ready = consumers_all(ready);  // warps that meet at barriers leave together
+        if (!ready) break;
         const Unit u = unit_records[k & 1];
         __syncwarp();
         if (lane == 0) mbar_arrive(unit_empty + 8 * (k & 1));
@@ -426,7 +442,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
 
         for (int j = turn; j < u.steps && !dead; j += turns) {
             const uint32_t n = done + j, st = n & (p.stages - 1);
-            if (!phase_wait(full + 8 * st, n / p.stages & 1, p.status)) {
+            if (!phase_wait(full + 8 * st, n / p.stages & 1, p.status, stop)) {
                 dead = true;
                 break;
             }

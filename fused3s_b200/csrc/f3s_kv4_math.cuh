@@ -17,6 +17,7 @@
 namespace f3s {
 
 constexpr uint64_t kAttendTimeoutNs = 5ull * 1000 * 1000 * 1000;
+constexpr uint64_t kDrainNs = 100ull * 1000 * 1000;
 constexpr float kNoReference = -3.0e38f;  // finite: a weight against it is 0, not NaN
 constexpr float kRescaleAt = 8.f;
 
@@ -100,23 +101,34 @@ __device__ __forceinline__ void lds_words(const uint8_t* p, uint32_t (&w)[N]) {
     }
 }
 
-// Waits for a phase of an mbarrier, by a whole warp; bounded.  False: give up.
-static __device__ __noinline__ bool phase_wait_slow(uint32_t bar, uint32_t parity, int* status) {
+// Waits for a phase of an mbarrier, by a whole warp; bounded.  False: give up, which
+// `status` reports and `stop` tells the waits that come after (the launch's own word,
+// or a plan's status: an error that an earlier launch left elsewhere stops nothing).
+static __device__ __noinline__ bool phase_wait_slow(uint32_t bar, uint32_t parity, int* status, int* stop) {
     const uint64_t t0 = global_timer_ns();
     for (;;) {
 #pragma unroll 1
         for (int i = 0; i < 64; ++i)
             if (mbar_try_wait(bar, parity)) return true;
-        if (load_volatile(status) == F3S_ERR_TIMEOUT) return false;
+        if (load_volatile(stop) == F3S_ERR_TIMEOUT) return false;
         if (global_timer_ns() - t0 > kAttendTimeoutNs) {
             atomicExch(status, F3S_ERR_TIMEOUT);
+            atomicExch(stop, F3S_ERR_TIMEOUT);
             return false;
         }
     }
 }
-__device__ __forceinline__ bool phase_wait(uint32_t bar, uint32_t parity, int* status) {
+__device__ __forceinline__ bool phase_wait(uint32_t bar, uint32_t parity, int* status, int* stop) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, phase_wait_slow(bar, parity, status));
+    return __all_sync(0xffffffffu, phase_wait_slow(bar, parity, status, stop));
+}
+
+// Lets the copies of ring steps first ... end - 1 land (stages bars apart 8 bytes), for
+// a limited time: shared memory is neither reused nor given up while they are in flight.
+static __device__ __noinline__ void ring_drain(uint32_t bars, uint32_t stages, uint32_t first, uint32_t end) {
+    for (uint32_t l = first; l < end; ++l)
+        if (!mbar_try_wait(bars + 8 * (l % stages), l / stages & 1))
+            mbar_drain(bars + 8 * (l % stages), l / stages & 1, kDrainNs);
 }
 
 // CH consecutive channels of a query row in O's type.

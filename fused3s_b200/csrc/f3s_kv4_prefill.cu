@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         bool unset = true;
         for (int j = 0; j < steps; ++j) {
             const int b = j & 1;
-            ok = ok && phase_wait(s_full + 8 * b, j >> 1 & 1, p.status);
+            ok = ok && phase_wait(s_full + 8 * b, j >> 1 & 1, p.status, p.status);
             if (pair_any(!ok)) {  // both halves leave together
                 ok = false;
                 break;
@@ -267,7 +267,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 den = mul2(den, pair(down, down));
                 off = mul2(off, pair(down, down));
                 if (j > 0) {  // O, once the products so far are in it: half of its columns each
-                    ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status) && ok;
+                    ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status, p.status) && ok;
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         }
         // ---- the result
         if (ok && steps > 0) {
-            ok = phase_wait(kv_empty + 8 * ((steps - 1) & 1), (steps - 1) >> 1 & 1, p.status);
+            ok = phase_wait(kv_empty + 8 * ((steps - 1) & 1), (steps - 1) >> 1 & 1, p.status, p.status);
             tc_fence_after();
         }
         {
@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         if (steps > 0) load(id);
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1;
-            ok = phase_wait(kv_empty + 8 * b, (j >> 1 & 1) ^ 1, p.status);
+            ok = phase_wait(kv_empty + 8 * b, (j >> 1 & 1) ^ 1, p.status, p.status);
             if (!ok) break;
             uint8_t* ks = smem + C::K + b * C::K_BYTES;
             uint8_t* vs = smem + C::V + b * C::V_BYTES;
@@ -398,10 +398,11 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         }
     } else if (warp == kRowWarps + kCodeWarps && live && steps > 0) {
         // ------------------------------------------------------------ products
-        ok = phase_wait(q_full, 0, p.status);
+        uint32_t last = 0, last_parity = 0;  // what the last products issued arrive on
+        ok = phase_wait(q_full, 0, p.status, p.status);
         auto weigh = [&](int j) {  // O += P V of step j
             const int b = j & 1;
-            ok = phase_wait(p_full + 8 * b, j >> 1 & 1, p.status);
+            ok = phase_wait(p_full + 8 * b, j >> 1 & 1, p.status, p.status);
             if (!ok) return;
             tc_fence_after();
             if (lane == 0) {
@@ -413,11 +414,13 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 }
                 mma_commit(kv_empty + 8 * b);  // K, V, the tokens' numbers and P are free, O is the step's
             }
+            last = kv_empty + 8 * b;
+            last_parity = j >> 1 & 1;
             __syncwarp();
         };
         for (int j = 0; j < steps && ok; ++j) {
             const int b = j & 1;
-            ok = phase_wait(kv_full + 8 * b, j >> 1 & 1, p.status);
+            ok = phase_wait(kv_full + 8 * b, j >> 1 & 1, p.status, p.status);
             if (!ok) break;
             tc_fence_after();
             if (lane == 0) {
@@ -428,10 +431,14 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                            mma_f16_shape(kTileRows, kStepTokens), k > 0);
                 mma_commit(s_full + 8 * b);
             }
+            last = s_full + 8 * b;
+            last_parity = j >> 1 & 1;
             __syncwarp();
             if (j > 0) weigh(j - 1);
         }
         if (ok) weigh(steps - 1);
+        // tensor and shared memory are given up after the products
+        if (last) mbar_drain(last, last_parity, kDrainNs);
     }
     __syncthreads();
     if (warp == kRowWarps + kCodeWarps) {
