@@ -397,8 +397,13 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
         p.splits = reinterpret_cast<f3s::Kv4Split*>(base + L.splits);
         units = std::max(units, L.items_cap);
     }
-    // one block per 1024 tokens or items, a block per SM at most
-    const int64_t blocks = std::min<int64_t>((units + 1023) / 1024, f3s::num_sms_of_current_device());
+    // One block per 1024 tokens or items, a block per SM at most.  Every block reads
+    // where the free list begins and the first one writes where it goes on: one block
+    // where that is the same word, since blocks do not wait for each other (41 prompts,
+    // 47,677 tokens: 79 us in place, 6.1 apart).
+    const int64_t blocks = d_free_begin_out == d_free_begin
+                               ? 1
+                               : std::min<int64_t>((units + 1023) / 1024, f3s::num_sms_of_current_device());
     f3s::k_block_tables<<<(unsigned)blocks, f3s::kBtThreads, 0, (cudaStream_t)stream>>>(p);
     F3S_LAUNCH_CHECK();
     return F3S_SUCCESS;

@@ -458,9 +458,9 @@ int f3s_kv4_load(const void* d_pages, int32_t num_pages, int32_t kv_heads, int32
  *   d_positions[num_tokens]            position of each new token in its request
  *   d_slots[num_tokens]                its slot (table entry * 16 + position % 16)
  *   d_free_begin_out[1]                the first page that is still free
- * (d_free_begin_out may be d_free_begin's memory only for a call that is not
- * repeated.)  num_tokens is the capacity of the token arrays; entries behind
- * the last new token get slot -1 and position 0.
+ * (d_free_begin_out may be d_free_begin's memory, for a call that is not
+ * repeated; one block then does the work.)  num_tokens is the capacity of the
+ * token arrays; entries behind the last new token get slot -1 and position 0.
  * heads, kv_heads: attention heads the plan is made for (0, 0: no plan).
  * d_plan: f3s_block_tables_workspace_size bytes, 16-byte aligned, also this
  * call's workspace (f3s_workspace_status); the call sets its status:

@@ -1,10 +1,13 @@
 """Calls of the 4-bit K / V operators as a program makes them: after an error,
 from several threads, in several captured graphs, in place, beside other
 kernels."""
+import random
+
 import pytest
 import torch
 
 import fused3s_b200 as F
+import kv4_ref as R
 import test_kv4 as T
 from fused3s_b200 import _lib, kv4
 
@@ -28,3 +31,33 @@ def test_an_earlier_timeout_stops_no_later_forward(lib, heads):
         F.fused3s_forward_kv4(q, cache, fmt, check_status=True)
     assert e.value.status == _lib.F3S_ERR_TIMEOUT
     F.fused3s_forward_kv4(q, cache, fmt, check_status=True)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads", [(0, 0), (32, 8)])
+def test_block_tables_in_place(lib, heads, kv_heads):
+    """The free list's first page updated in place, for more tokens than one block
+    takes, while another stream keeps the SMs busy."""
+    rng = random.Random(3)
+    lengths = [(rng.choice([0, rng.randrange(3000)]), rng.randrange(400, 1777)) for _ in range(41)]
+    tables, free, begin, _ = T.make_tables(lengths, 2)
+    tokens, requests, width = sum(n for _, n in lengths), len(lengths), len(tables[0])
+    want = R.block_tables([c for c, _ in lengths], [n for _, n in lengths], tables, free, begin, tokens)
+    size = lib.f3s_block_tables_workspace_size(requests, tokens, heads, kv_heads)
+    context, new, free = T.i32([c for c, _ in lengths]), T.i32([n for _, n in lengths]), T.i32(free)
+    offsets, positions, slots = (torch.empty(n, dtype=torch.int32, device="cuda") for n in (requests + 1, tokens, tokens))
+    plan = torch.empty(size, dtype=torch.uint8, device="cuda")
+    busy, side = torch.randn(4096, 4096, device="cuda"), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        table, word = T.i32(tables), T.i32([begin])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            busy @ busy
+        st = lib.f3s_block_tables(context.data_ptr(), new.data_ptr(), requests, table.data_ptr(), width, width,
+                                  free.data_ptr(), free.numel(), word.data_ptr(), tokens, heads, kv_heads,
+                                  offsets.data_ptr(), positions.data_ptr(), slots.data_ptr(), word.data_ptr(),
+                                  plan.data_ptr(), size, torch.cuda.current_stream().cuda_stream)
+        assert st == 0 and lib.f3s_workspace_status(plan.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        got = (offsets.tolist(), positions.tolist(), slots.tolist(), table.tolist(), word.item())
+        assert got == want
