@@ -31,6 +31,7 @@ build_block_tables and attention_kv4 in the block tables (status()).
 from __future__ import annotations
 
 import functools
+import threading
 from typing import Optional, Tuple
 
 import torch
@@ -58,20 +59,23 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 _STATUS = {}  # one status word per device for store, load and the graph forward
+_STATUS_LOCK = threading.Lock()
 
 
 def _status(device: torch.device) -> torch.Tensor:
     """The device's status word: kernels only set it where it is 0, so all streams
-    and captured graphs share it.  Made before any capture, with the first cache."""
-    ws = _STATUS.get(device.index)
-    if ws is None:
-        with torch.cuda.device(device):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("make the device's first KV4Cache before capturing a CUDA graph")
-            ws = torch.zeros(256, dtype=torch.uint8, device=device)
-            torch.cuda.current_stream(device).synchronize()
-        _STATUS[device.index] = ws
-    return ws
+    and captured graphs share it.  Made before any capture, with the first cache,
+    once whichever threads ask for it."""
+    with _STATUS_LOCK:
+        ws = _STATUS.get(device.index)
+        if ws is None:
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("make the device's first KV4Cache before capturing a CUDA graph")
+                ws = torch.zeros(256, dtype=torch.uint8, device=device)
+                torch.cuda.current_stream(device).synchronize()
+            _STATUS[device.index] = ws
+        return ws
 
 
 class KV4Cache:
@@ -79,7 +83,7 @@ class KV4Cache:
     16 * head_dim + 128], contiguous, on a CUDA device.  Wraps the tensor; a
     page of zeros holds zeros."""
 
-    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim", "device", "status_ptr")
+    __slots__ = ("pages", "num_pages", "kv_heads", "head_dim", "device", "status_word", "status_ptr")
 
     def __init__(self, pages: torch.Tensor):
         if pages.dtype != torch.uint8 or pages.dim() != 3:
@@ -96,7 +100,8 @@ class KV4Cache:
         self.head_dim = _RECORDS[record]
         self.pages = pages
         self.device = pages.device
-        self.status_ptr = _status(self.device).data_ptr()
+        self.status_word = _status(self.device)
+        self.status_ptr = self.status_word.data_ptr()
 
 
 def empty_kv4_cache(num_pages: int, kv_heads: int, head_dim: int, device=None) -> KV4Cache:

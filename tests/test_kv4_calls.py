@@ -1,7 +1,10 @@
 """Calls of the 4-bit K / V operators as a program makes them: after an error,
 from several threads, in several captured graphs, in place, beside other
 kernels."""
+import contextlib
 import random
+import threading
+import time
 
 import pytest
 import torch
@@ -12,6 +15,45 @@ import test_kv4 as T
 from fused3s_b200 import _lib, kv4
 
 gpu = pytest.mark.gpu
+
+
+def test_first_caches_of_two_threads_share_one_status_word(monkeypatch):
+    """Two threads that make a device's first cache get the same word, which lives on
+    (the device's calls stand-ins that give way to the other thread)."""
+    made = []
+
+    class Stream:
+        def synchronize(self):
+            time.sleep(0.05)
+
+    def zeros(n, dtype=None, device=None):
+        made.append(torch.empty(n, dtype=dtype))
+        time.sleep(0.05)
+        return made[-1]
+
+    monkeypatch.setattr(kv4, "_STATUS", {})
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream())
+    monkeypatch.setattr(torch, "zeros", zeros)
+    device, got, both = torch.device("cuda", 0), [None, None], threading.Barrier(2)
+
+    def first_cache(i):
+        both.wait()
+        got[i] = kv4._status(device)
+
+    threads = [threading.Thread(target=first_cache, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and got[0] is made[0] and got[1] is made[0] and kv4._STATUS[0] is made[0]
+
+
+@gpu
+def test_a_cache_keeps_its_status_word(lib):
+    cache = F.empty_kv4_cache(2, 1, 64)
+    assert cache.status_word.data_ptr() == cache.status_ptr and cache.status_word is kv4._STATUS[cache.device.index]
 
 
 @gpu
