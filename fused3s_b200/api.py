@@ -246,7 +246,9 @@ def generate_balanced_window_order(fmt: BlockSparseFormat) -> torch.Tensor:
     lib = _lib.load()
     device = fmt.window_offsets.device
     order = torch.empty(max(fmt.num_row_windows, 1), dtype=torch.int32, device=device)
-    ws = _WS.get(device, "order", lib.f3s_window_order_workspace_size(fmt.num_row_windows))
+    # scratch of this call's own, from torch's allocator: captured graphs whose sorts run
+    # at the same time, or that outlive a larger graph's, share none of it
+    ws = torch.empty(lib.f3s_window_order_workspace_size(fmt.num_row_windows), dtype=torch.uint8, device=device)
     with torch.cuda.device(device):
         st = lib.f3s_window_order(_ptr(fmt.window_offsets), fmt.num_row_windows, _ptr(order), _ptr(ws),
                                   ws.numel(), _stream_ptr(device))

@@ -12,7 +12,7 @@ import torch
 import fused3s_b200 as F
 import kv4_ref as R
 import test_kv4 as T
-from fused3s_b200 import _lib, kv4
+from fused3s_b200 import _lib, api, kv4
 
 gpu = pytest.mark.gpu
 
@@ -48,6 +48,58 @@ def test_first_caches_of_two_threads_share_one_status_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(made) == 1 and got[0] is made[0] and got[1] is made[0] and kv4._STATUS[0] is made[0]
+
+
+class OrderLibrary:
+    """Stands in for libfused3s.so: notes the scratch of each sort."""
+
+    def __init__(self):
+        self.scratch = []
+
+    def f3s_window_order_workspace_size(self, n):
+        return 1000 + n
+
+    def f3s_window_order(self, offsets, n, order, ws, ws_bytes, stream):
+        self.scratch.append((ws, ws_bytes))
+        return 0
+
+
+def test_the_order_of_windows_keeps_no_scratch(monkeypatch):
+    """Nothing that a captured sort writes to stays behind for the next one to share or replace."""
+    fake = OrderLibrary()
+    monkeypatch.setattr(api._lib, "load", lambda: fake)
+    monkeypatch.setattr(api, "_stream_ptr", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "device", lambda device: contextlib.nullcontext())
+    monkeypatch.setattr(api, "_WS", api._WorkspaceCache())
+    for n in (70, 7000):
+        offsets = torch.zeros(n + 1, dtype=torch.int32)
+        fmt = F.BlockSparseFormat(n, offsets, torch.zeros(0, dtype=torch.int32), 16 * n)
+        assert api.generate_balanced_window_order(fmt).shape == (n,)
+    assert [size for _, size in fake.scratch] == [1070, 8000] and not api._WS._ws
+
+
+@gpu
+def test_captured_forwards_sort_their_windows_apart(lib):
+    """Forwards without an order, of graphs of three sizes, captured one after another
+    and replayed at the same time on streams of their own."""
+    d, heads, cases = 64, 2, []
+    for n, edges in ((3000, 20000), (40000, 90000), (9000, 50000)):
+        _, fmt = T.graph_case(n, heads, d, 5, edges=edges)
+        cache = T.filled_cache(fmt.num_row_windows, heads, d, 4)
+        q = T.randn((n, heads, d), 5, torch.float16).cuda()
+        want = F.fused3s_forward_kv4(q, cache, fmt, scale=0.125, check_status=True)
+        graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(want)
+        with torch.cuda.graph(graph):
+            F.fused3s_forward_kv4(q, cache, fmt, scale=0.125, out=out)
+        cases.append((graph, out, want, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, out, _, stream in cases:
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, out, want, _ in cases)
 
 
 @gpu
