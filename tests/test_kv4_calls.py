@@ -91,15 +91,15 @@ def test_captured_forwards_sort_their_windows_apart(lib):
         graph, out = torch.cuda.CUDAGraph(), torch.zeros_like(want)
         with torch.cuda.graph(graph):
             F.fused3s_forward_kv4(q, cache, fmt, scale=0.125, out=out)
-        cases.append((graph, out, want, torch.cuda.Stream()))
+        cases.append((graph, out, want, torch.cuda.Stream(), (fmt, cache, q)))  # what the graph reads lives as long
     torch.cuda.synchronize()
     for _ in range(20):
-        for graph, out, _, stream in cases:
+        for graph, out, _, stream, _ in cases:
             with torch.cuda.stream(stream):
                 out.zero_()
                 graph.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(out, want) for _, out, want, _ in cases)
+        assert all(torch.equal(out, want) for _, out, want, _, _ in cases)
 
 
 @gpu
