@@ -362,11 +362,15 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                 const uint32_t h0 = pack_half2(a[0], a[1]), h1 = pack_half2(a[2], a[3]);
                 pb[nt][0] = movmatrix_t(h0);
                 pb[nt][1] = movmatrix_t(h1);
+                const float2 r0 = half2_floats(h0), r1 = half2_floats(h1);
                 if constexpr (PRECISE) {
-                    const float2 r0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                    const float2 r1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
                     pl[nt][0] = movmatrix_t(pack_half2(a[0] - r0.x, a[1] - r0.y));
                     pl[nt][1] = movmatrix_t(pack_half2(a[2] - r1.x, a[3] - r1.y));
+                } else {  // the same weights in every sum (f3s_kv4_math.cuh)
+                    a[0] = r0.x;
+                    a[1] = r0.y;
+                    a[2] = r1.x;
+                    a[3] = r1.y;
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {

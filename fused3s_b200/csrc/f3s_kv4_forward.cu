@@ -585,12 +585,14 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                     for (int c = 0; c < 2; ++c) {
                         const float2 y = unpair(x[k2][r][c]);
                         const float2 a = make_float2(exp2_approx(y.x), exp2_approx(y.y));
-                        const uint64_t a2 = pair(a.x, a.y);
+                        uint64_t a2 = pair(a.x, a.y);
                         pa[2 * c + r] = pack_half2(a.x, a.y);
+                        const float2 b = half2_floats(pa[2 * c + r]);
                         if constexpr (PRECISE) {
-                            const float2 b = half2_floats(pa[2 * c + r]);
                             const float2 d = unpair(fma2(pair(b.x, b.y), pair(-1.f, -1.f), a2));
                             pl[2 * c + r] = pack_half2(d.x, d.y);
+                        } else {  // the same weights in every sum
+                            a2 = pair(b.x, b.y);
                         }
                         den[r] = fma2(a2, c ? ri.y : ri.x, den[r]);
                         off[r] = fma2(a2, c ? vz.y : vz.x, off[r]);

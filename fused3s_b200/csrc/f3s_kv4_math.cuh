@@ -258,8 +258,13 @@ __device__ __forceinline__ void merge_rows(int count, int subs, int tq, int live
 }
 
 // Whether the weights are multiplied in full (fp16 and what its rounding drops) or
-// rounded to fp16.  Rounded, a result's error doubles where it is written in fp16
-// (4.0e-4 against 2.1e-4 of the result, 131,057 nodes) and is lost in bf16's.
+// rounded to fp16.  Rounded weights go into all three sums: then a result is the
+// average that these weights make, and a rounding moves it by at most 2^-11 of the
+// values' distance from it.  (With unrounded weights in the sums of zeros and of
+// weights, a rounding would act on codes, 0 ... 15, whose sums are far larger than
+// their difference, the result: 3e-4 of V's size for 3,000 tokens of +1 and -1 that
+// weigh alike, where the result is 2e-2.)  Rounded, a result's error doubles
+// where it is written in fp16 (4.0e-4 against 2.1e-4 of the result, 131,057 nodes).
 inline bool weights_in_full(int o_dtype) { return o_dtype != F3S_OUT_BF16; }
 
 // Arguments that the attentions share.

@@ -229,12 +229,10 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                         const float2 v = unpair(x[i]), w = unpair(add2(x[i], mref2));
                         most = fmaxf(most, fmaxf(v.x, v.y));
                         const float2 a = make_float2(exp2_approx(w.x), exp2_approx(w.y));
-                        const uint64_t a2 = pair(a.x, a.y);
                         hi[2 * c + i] = pack_half2(a.x, a.y);
-                        if constexpr (PRECISE) {
-                            const float2 h = half2_floats(hi[2 * c + i]);
-                            lo[2 * c + i] = pack_half2(a.x - h.x, a.y - h.y);
-                        }
+                        const float2 h = half2_floats(hi[2 * c + i]);
+                        if constexpr (PRECISE) lo[2 * c + i] = pack_half2(a.x - h.x, a.y - h.y);
+                        const uint64_t a2 = PRECISE ? pair(a.x, a.y) : pair(h.x, h.y);  // the same weights in every sum
                         d = fma2(a2, i ? ri.y : ri.x, d);
                         o = fma2(a2, i ? y.y : y.x, o);
                     }

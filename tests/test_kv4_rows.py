@@ -46,6 +46,75 @@ def star(n):
     return F.convert_csr_to_block_sparse(n, row_ptr, np.concatenate([np.arange(n), np.zeros(n - 1)]).astype(np.int32))
 
 
+# ------------------------------------------------- weights that round alike --
+
+def alike(n, kv_heads, d, seed):
+    """K and V of n tokens: every sixteenth token scores L above the others, L
+    such that the others' weight lies 0.49 of an fp16 step above an fp16 number;
+    V of +1 and -1, so that every row has the same scale.  And q's value, the
+    scale that makes L, L."""
+    level = 1 - math.log2(1.5 + 0.49 * 2.0 ** -10)
+    k = torch.zeros(n, kv_heads, d)
+    k[::16] = 1.0
+    v = torch.where(T.randn((n, kv_heads, d), seed) > 0, 1.0, -1.0)
+    one = 15 * float(torch.tensor(1 / 15).half())  # what a row of ones stands for
+    return k.half().cuda(), v.half().cuda(), 0.125, level * math.log(2) / (d * 0.125 * one), level
+
+
+def check_alike(got, k, v, visible, level, out_dtype):
+    """got [rows, d] against 64 bits.
+
+    Rounding the weights to fp16 (off by e <= 2^-11 of them, the same for tokens of
+    the same score) moves the result by at most 2 e p (1 - p) |A - B|, with p the
+    share of the high tokens and A, B the means of V over the high and the other
+    tokens -- if the same weights are used in every sum.  The sums of codes times
+    scales reach 2 (codes 0 ... 15 of a span of 2) and are off by 64 steps of
+    2^-23 and one per product of 16 tokens.  The result is rounded once."""
+    high = torch.arange(k.shape[0]) % 16 == 0
+    weight = torch.where(high, 2.0 ** level, 1.0).double() * visible
+    share = weight / weight.sum(-1, keepdim=True)
+    want = share @ v
+    p = (share * high).sum(-1, keepdim=True)
+    a, b = (share * high) @ v / p, (share * ~high) @ v / (1 - p)
+    tol = 2 * 2.0 ** -11 * p * (1 - p) * (a - b).abs() if out_dtype == torch.bfloat16 else 0.0
+    tol = tol + 2 * (64 + k.shape[0] / 16) * 2.0 ** -23 + HALF_STEP[out_dtype] * want.abs()
+    R.assert_close(got, want, tol)
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,new,height", [(2, 1, 8), (2, 30, 16), (2, 150, 128)])
+def test_attention_weights_that_round_alike(lib, heads, new, height, d, out_dtype):
+    n = 3000 + new
+    cache, bt, rows = paged([(3000, new)], heads, 1, d, 5)
+    assert tile_rows(bt) == height
+    k, v, q, scale, level = alike(n, 1, d, 7)
+    F.store_kv4(k, v, slots_of(rows[0], n), cache, check_status=True)
+    Q = torch.full((new, heads, d), q, dtype=torch.bfloat16, device="cuda")
+    o = F.attention_kv4(Q, cache, bt, scale=scale, out_dtype=out_dtype, check_status=True)
+    k, v = values(cache, rows[0], n)
+    visible = torch.arange(n)[None, :] <= (3000 + torch.arange(new))[:, None]
+    for h in range(heads):
+        check_alike(o[:, h], k, v, visible, level, out_dtype)
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("heads,d", [(1, 64), (2, 64), (4, 64), (4, 128)])
+def test_graph_weights_that_round_alike(lib, heads, d, out_dtype):
+    n = 3008
+    fmt = star(n)
+    k, v, q, scale, level = alike(n, 1, d, 8)
+    cache = F.empty_kv4_cache(fmt.num_row_windows, 1, d)
+    F.store_kv4(k, v, torch.arange(n, dtype=torch.int32, device="cuda"), cache, check_status=True)
+    Q = torch.full((n, heads, d), q, dtype=torch.bfloat16, device="cuda")
+    o = F.fused3s_forward_kv4(Q, cache, fmt, scale=scale, out_dtype=out_dtype, check_status=True)
+    k, v = values(cache, list(range(n // 16)), n)
+    for h in range(heads):
+        check_alike(o[:16, h], k, v, torch.ones(16, n), level, out_dtype)
+
+
 # ----------------------------------------------- scores beyond whole steps --
 
 @gpu
