@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(m, ref[nt][j]);
+                    m = fmaxf(m - kTopWeight, ref[nt][j]);
                     const float c = exp2_approx(ref[nt][j] - m);
                     ref[nt][j] = m;
                     den[nt][j] *= c;

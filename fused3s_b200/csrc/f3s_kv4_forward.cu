@@ -552,11 +552,11 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                     float up;  // the reference moves up by this
                     if (unset >> r & 1) {  // nothing seen so far: the sums are 0, whatever they are scaled by
-                        up = m > -INFINITY ? m : 0.f;
+                        up = m > -INFINITY ? m - kTopWeight : 0.f;
                         down[r] = 1.f;
                         if (m > -INFINITY) unset &= ~(1u << r);
                     } else {
-                        up = fmaxf(m, 0.f);
+                        up = fmaxf(m - kTopWeight, 0.f);
                         down[r] = exp2_approx(-up);
                     }
                     const uint64_t minus = pair(-up, -up), by = pair(down[r], down[r]);

@@ -3,12 +3,15 @@
 //
 // With k_t = s_t (u_t - z_t) and v_t = r_t (w_t - y_t) (scales s, r, zeros z, y, codes u, w):
 //   x_t = scale log2(e) s_t (q . u_t - z_t sum(q))                 the score, in powers of two
-//   a_t = 2^(x_t + log2 r_t - R),  R >= x_t + log2 r_t - 8          the weight times V's scale
+//   a_t = 2^(x_t + log2 r_t - R),  R >= x_t + log2 r_t - 15         the weight times V's scale
 //   O   = (sum a_t w_t - sum a_t y_t) / sum a_t / r_t
 // so the two matrix products read whole numbers 0 ... 15 and every scale is
 // applied to a score, not to a value.  R is a running reference per query row:
-// it moves (and the sums are rescaled) only when a weight would pass 2^8, which
-// one vote per step decides.
+// it moves (and the sums are rescaled) only when a weight would pass 2^15, which
+// one vote per step decides, and then leaves the largest weight at 2^7: of the
+// fp16 numbers that P is held in, those with full precision reach from 2^-14 to
+// 2^16, and what a weight loses below that is 2^-25, 2^-32 of the largest.  (With
+// the largest at 1 a thousand tokens that weigh 2^-20 each moved fp32 results by 3e-5.)
 #pragma once
 #include <cuda_bf16.h>
 #include "f3s_internal.cuh"
@@ -19,7 +22,8 @@ namespace f3s {
 constexpr uint64_t kAttendTimeoutNs = 5ull * 1000 * 1000 * 1000;
 constexpr uint64_t kDrainNs = 100ull * 1000 * 1000;
 constexpr float kNoReference = -3.0e38f;  // finite: a weight against it is 0, not NaN
-constexpr float kRescaleAt = 8.f;
+constexpr float kRescaleAt = 15.f;  // log2 of the largest weight that a reference is kept for, below fp16's end
+constexpr float kTopWeight = 7.f;   // and of the largest weight when a reference is set
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),

@@ -13,7 +13,7 @@
 //   warp 12     issues S = Q K^T into one of two S buffers in tensor memory, and
 //               O += P V with P read from tensor memory
 // S of a step runs while the weights of the one before are worked out, and two
-// blocks share an SM.  A weight's reference moves when it passes 2^8; then the
+// blocks share an SM.  A row's reference moves when a weight passes 2^15; then the
 // rows' warps rescale O in tensor memory themselves, once the products before are
 // done.
 //
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             uint32_t hi[16], lo[PRECISE ? 16 : 1];  // P, two tokens each, and what its rounding drops
             // Weights and sums against the reference as it stands; the largest score.  A score
             // is rounded before the reference is taken off, so that no weight passes
-            // 1 once the reference is the largest score, however large that is.
+            // 2^8 once the reference is the largest score less 7, however large that is.
             auto weigh_row = [&](auto hides, uint64_t& den_out, uint64_t& off_out) {
                 constexpr bool HIDES = decltype(hides)::value;
                 float most = -INFINITY;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 pair_sync();
                 const float m = fmaxf(most, largest[(half ^ 1) * kTileRows + r]);
                 const float before = minus_ref;
-                if (m > -INFINITY) minus_ref = unset ? -m : fminf(minus_ref, -m);
+                if (m > -INFINITY) minus_ref = unset ? kTopWeight - m : fminf(minus_ref, kTopWeight - m);
                 const float down = unset ? 1.f : exp2_approx(minus_ref - before);
                 unset = unset && !(m > -INFINITY);
                 den = mul2(den, pair(down, down));

@@ -115,6 +115,79 @@ def test_graph_weights_that_round_alike(lib, heads, d, out_dtype):
         check_alike(o[:16, h], k, v, torch.ones(16, n), level, out_dtype)
 
 
+# --------------------------------------------- one token above all others --
+
+LOW = 24 - math.log2(22.49)  # the others' weight, 2^-LOW, lies midway between two numbers 2^-24 apart
+
+
+def one_above(n, kv_heads, d):
+    """K and V of n tokens: the first scores LOW above the others and has V = -1, the others +1."""
+    k, v = torch.zeros(n, kv_heads, d), torch.ones(n, kv_heads, d)
+    k[0], v[0] = 1.0, -1.0
+    one = 15 * float(torch.tensor(1 / 15).half())
+    return k.half().cuda(), v.half().cuda(), 0.125, LOW * math.log(2) / (d * 0.125 * one)
+
+
+def check_one_above(got, v, seen, d):
+    """got [rows, d] (fp32) of rows that see `seen` tokens.
+
+    The others' share of the weights is s; their scores, LOW ln 2 below the first,
+    are off by 3 LOW ln 2 (d / 16 + 4) 2^-22 in numerator and denominator each
+    (codes and zeros apart, as in kv4_ref.tolerance), which moves the result by 2 s
+    times that.  A weight in two fp16 parts is off by 2^-21 of it or by half of the
+    smallest fp16 number, 2^-25, where the largest weight is 2^7 or more: 2^-32
+    of it; V's values are 2 apart.  Reciprocals and sums add 64 steps of 2^-23."""
+    low = (seen - 1).double() * 2.0 ** -LOW
+    one = float(v[1, 0])
+    want = one * (low - 1) / (low + 1)
+    s = low / (low + 1)
+    tol = 2 * s * (2 * 3 * LOW * math.log(2) * (d / 16 + 4) * 2.0 ** -22 + 2.0 ** -21)
+    tol = tol + 2 * seen.double() * 2.0 ** -32 + 2 * 64 * 2.0 ** -23
+    R.assert_close(got, want[:, None].expand(-1, d), tol[:, None].expand(-1, d))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_one_token_above_all_others(lib, d):
+    """Prompts whose tiles walk 100 pages and more in one piece."""
+    context, new, heads = 8000, 2048, 8
+    n = context + new
+    cache, bt, rows = paged([(context, new)], heads, heads, d, 5)
+    assert tile_rows(bt) == 128
+    k, v, q, scale = one_above(n, heads, d)
+    F.store_kv4(k, v, slots_of(rows[0], n), cache, check_status=True)
+    Q = torch.full((new, heads, d), q, dtype=torch.bfloat16, device="cuda")
+    o = F.attention_kv4(Q, cache, bt, scale=scale, out_dtype=torch.float32, check_status=True)
+    _, v = values(cache, rows[0], 16)
+    for h in (0, heads - 1):
+        check_one_above(o[:, h], v, context + torch.arange(new) + 1, d)
+
+
+@gpu
+@pytest.mark.parametrize("heads,d", [(1, 64), (4, 128)])
+def test_graph_one_token_above_all_others(lib, heads, d):
+    """A window that sees 2,500 blocks in one piece (the caller's estimate of the blocks sets its length)."""
+    n = 40000
+    fmt = star(n)
+    k, v, q, scale = one_above(n, 1, d)
+    cache = F.empty_kv4_cache(fmt.num_row_windows, 1, d)
+    F.store_kv4(k, v, torch.arange(n, dtype=torch.int32, device="cuda"), cache, check_status=True)
+    Q = torch.full((16, heads, d), q, dtype=torch.float16, device="cuda")
+    o = torch.empty((16, heads, d), device="cuda")
+    order, blocks = T.i32([0]), 6 * 160 * 2500
+    size = lib.f3s_kv4_forward_scratch_size(1, blocks, heads, 1, d)
+    scratch = torch.empty(size, dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(256, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    st = lib.f3s_kv4_forward(Q.data_ptr(), _lib.F3S_OUT_F16, cache.pages.data_ptr(), cache.num_pages, o.data_ptr(),
+                             _lib.F3S_OUT_F32, fmt.window_offsets.data_ptr(), fmt.cols_ptr, order.data_ptr(), 1, blocks,
+                             n, heads, 1, d, scale, 0, 16, ws.data_ptr(), 256, scratch.data_ptr(), size, stream)
+    assert st == 0 and lib.f3s_workspace_status(ws.data_ptr(), stream) == 0
+    _, v = values(cache, [0], 16)
+    for h in range(heads):
+        check_one_above(o[:, h], v, torch.full((16,), n), d)
+
+
 # ----------------------------------------------- scores beyond whole steps --
 
 @gpu
