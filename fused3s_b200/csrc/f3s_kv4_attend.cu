@@ -131,17 +131,17 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
     for (int i = 0; i < min(steps, STAGES); ++i) issue(i);
 
     // ---- Q: rows g of each n-tile, channels t * D / 4 ..., as fp16 times a
-    // power of two that brings the tile's largest to [2^9, 2^10); channels
+    // power of two that brings the row's largest to [2^9, 2^10); channels
     // whose codes come in units of 2^-24 another 2^4
     uint32_t qf[NT][W][4];
-    float qs[NT][2];  // sum of q (in the scores' unit) of rows 2t, 2t + 1
-    float unit_scale;
+    float qs[NT][2], qu[NT][2];  // rows 2t, 2t + 1: sum of q, and what a score's unit stands for
     {
-        float amax = 0.f;
+        float amax[NT], up2[NT], sums[NT];  // up2: what the power of two divides by
         uint4 raw[NT][W];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const int r = nt * 8 + g;
+            amax[nt] = 0.f;
             int64_t off = -1;
             const int row = it.row0 + r;
             if (row < it.rows) {
@@ -166,21 +166,20 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
                     }
                     a = fabsf(a);
                     b = fabsf(b);
-                    if (a < INFINITY) amax = fmaxf(amax, a);  // NaN and infinities stay what they are
-                    if (b < INFINITY) amax = fmaxf(amax, b);
+                    if (a < INFINITY) amax[nt] = fmaxf(amax[nt], a);  // NaN and infinities stay what they are
+                    if (b < INFINITY) amax[nt] = fmaxf(amax[nt], b);
                 }
             }
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-        // 2^(9 - floor(log2 amax)), kept within fp32's normal range
-        const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
-        const int up = min(max(9 - e, -120), 120);
-        const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-        unit_scale = p.scale * __uint_as_float((uint32_t)(127 - up) << 23);
-        float sums[NT];
-#pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            amax[nt] = fmaxf(amax[nt], __shfl_xor_sync(0xffffffffu, amax[nt], 1));
+            amax[nt] = fmaxf(amax[nt], __shfl_xor_sync(0xffffffffu, amax[nt], 2));
+            // 2^(9 - floor(log2 amax)), kept within fp32's normal range
+            const int e = amax[nt] > 0.f ? (int)(__float_as_uint(amax[nt]) >> 23) - 127 : 9;
+            const int up = min(max(9 - e, -120), 120);
+            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+            up2[nt] = __uint_as_float((uint32_t)(127 - up) << 23);
             float sum = 0.f;
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -213,6 +212,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         for (int nt = 0; nt < NT; ++nt) {
             qs[nt][0] = __shfl_sync(0xffffffffu, sums[nt], 8 * t);      // row 2t is summed in lanes 4 * 2t ...
             qs[nt][1] = __shfl_sync(0xffffffffu, sums[nt], 8 * t + 4);  // row 2t + 1
+            qu[nt][0] = p.scale * __shfl_sync(0xffffffffu, up2[nt], 8 * t);
+            qu[nt][1] = p.scale * __shfl_sync(0xffffffffu, up2[nt], 8 * t + 4);
         }
     }
 
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             const float2 va = __half22float2(*reinterpret_cast<const __half2*>(&sc.y));
             const float2 kb = __half22float2(*reinterpret_cast<const __half2*>(&sc.z));
             const float2 vb = __half22float2(*reinterpret_cast<const __half2*>(&sc.w));
-            const float fa = ka.x * 1048576.f * unit_scale, fb = kb.x * 1048576.f * unit_scale;  // 2^20: the codes' unit
+            const float fa = ka.x * 1048576.f, fb = kb.x * 1048576.f;  // 2^20: the codes' unit
             const float ra = va.x < kKv4MinScale ? kKv4MinScale : va.x;  // keeps a NaN
             const float rb = vb.x < kKv4MinScale ? kKv4MinScale : vb.x;
             const float la = log2_approx(ra), lb = log2_approx(rb);
@@ -288,7 +289,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float z = c < 2 ? ka.y : kb.y;
-                    x[k][nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], s[nt][c]), c < 2 ? fa : fb, c < 2 ? la : lb);
+                    x[k][nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], s[nt][c]), (c < 2 ? fa : fb) * qu[nt][c & 1], c < 2 ? la : lb);
                 }
         }
         // ---- masks: only where a page has tokens that some row must not see

@@ -354,14 +354,14 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
         const int kv_off = (head / p.group - u.head0 / p.group) * RB;  // in a page of a stage
         const int64_t row0 = (int64_t)(u.window - p.q_window_base) * 16 + g;  // lane (g, t): rows g and g + 8
 
-        // ---- Q as fp16 times a power of two that brings the tile's largest to
+        // ---- Q as fp16 times a power of two that brings the row's largest to
         // [2^9, 2^10); channels whose codes come in units of 2^-24 another 2^4.
         // Lane (g, t): channels t * D / 4 ... of its rows
-        uint64_t qs[2];  // sum of a row's q in the scores' unit, twice
-        float unit_scale;
+        uint64_t qs[2], qu[2];  // per row, twice: scale times the sum of q; what a score's unit stands for
         {
             uint4 raw[2][W];
-            uint32_t top = 0;
+            uint32_t top[2] = {0, 0};
+            uint64_t by[2][2];
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
                 const int64_t row = row0 + 8 * r;
@@ -376,34 +376,37 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 for (int w = 0; w < W; ++w) {
                     const uint32_t x[4] = {raw[r][w].x, raw[r][w].y, raw[r][w].z, raw[r][w].w};
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) top = max_pair(top, x[n] & 0x7fff7fffu, p.q_bf16);
+                    for (int n = 0; n < 4; ++n) top[r] = max_pair(top[r], x[n] & 0x7fff7fffu, p.q_bf16);
                 }
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) top = max_pair(top, __shfl_xor_sync(0xffffffffu, top, o), p.q_bf16);
-            const float2 two = q_floats(top, p.q_bf16);
-            float amax = fmaxf(two.x, two.y);
-            if (!(amax < INFINITY)) {  // an infinity: the largest of the others; it stays what it is
-                amax = 0.f;
-#pragma unroll 1
-                for (int i = 0; i < 2 * W * 4; ++i) {
-                    const int r = i / (W * 4), w = i / 4 % W, n = i % 4;
+            for (int r = 0; r < 2; ++r) {
+                top[r] = max_pair(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1), p.q_bf16);
+                top[r] = max_pair(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2), p.q_bf16);
+                const float2 two = q_floats(top[r], p.q_bf16);
+                float amax = fmaxf(two.x, two.y);
+                if (__any_sync(0xffffffffu, !(amax < INFINITY))) {  // an infinity: the largest of the others; it stays what it is
+                    amax = 0.f;
                     const int64_t row = row0 + 8 * r;
                     const uint32_t* at = reinterpret_cast<const uint32_t*>(static_cast<const uint16_t*>(p.q) + row * p.q_token +
                                                                            (int64_t)head * p.q_head + t * (D / 4));
-                    const uint32_t x = row < p.q_rows ? at[4 * w + n] : 0;
-                    const float2 y = q_floats(x, p.q_bf16);
-                    if (fabsf(y.x) < INFINITY) amax = fmaxf(amax, fabsf(y.x));
-                    if (fabsf(y.y) < INFINITY) amax = fmaxf(amax, fabsf(y.y));
+#pragma unroll 1
+                    for (int i = 0; i < W * 4; ++i) {
+                        const float2 y = q_floats(row < p.q_rows ? at[i] : 0, p.q_bf16);
+                        if (fabsf(y.x) < INFINITY) amax = fmaxf(amax, fabsf(y.x));
+                        if (fabsf(y.y) < INFINITY) amax = fmaxf(amax, fabsf(y.y));
+                    }
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                // 2^(9 - floor(log2 amax)), kept within fp32's normal range
+                const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
+                const int up = min(max(9 - e, -120), 120);
+                const float f = __uint_as_float((uint32_t)(up + 127) << 23);
+                const float unit = p.scale * __uint_as_float((uint32_t)(127 - up) << 23);
+                qu[r] = pair(unit, unit);
+                by[r][0] = pair(f * 16.f, f * 16.f);
+                by[r][1] = pair(f, f);
             }
-            // 2^(9 - floor(log2 amax)), kept within fp32's normal range
-            const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
-            const int up = min(max(9 - e, -120), 120);
-            const float f = __uint_as_float((uint32_t)(up + 127) << 23);
-            unit_scale = p.scale * __uint_as_float((uint32_t)(127 - up) << 23);
-            const uint64_t by[2] = {pair(f * 16.f, f * 16.f), pair(f, f)};
             float sum[4];  // the rows' sums, as a product with 1 (and 2^-4)
 #pragma unroll
             for (int w = 0; w < W; ++w) {
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                     const uint32_t x[4] = {raw[r][w].x, raw[r][w].y, raw[r][w].z, raw[r][w].w};
 #pragma unroll
                     for (int n = 0; n < 4; ++n) {
-                        const float2 y = q_floats(x[n], p.q_bf16), z = unpair(mul2(pair(y.x, y.y), by[n & 1]));
+                        const float2 y = q_floats(x[n], p.q_bf16), z = unpair(mul2(pair(y.x, y.y), by[r][n & 1]));
                         h[4 * r + n] = pack_half2(z.x, z.y);
                     }
                 }
@@ -425,9 +428,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 qsm[2 * w * 32 + lane] = make_uint4(h[0], h[4], h[1], h[5]);
                 qsm[(2 * w + 1) * 32 + lane] = make_uint4(h[2], h[6], h[3], h[7]);
             }
-            const float s0 = sum[0] * 9.5367431640625e-7f, s1 = sum[2] * 9.5367431640625e-7f;  // 2^-20
-            qs[0] = pair(s0, s0);
-            qs[1] = pair(s1, s1);
+            qs[0] = mul2(qu[0], pair(sum[0], sum[0]));
+            qs[1] = mul2(qu[1], pair(sum[2], sum[2]));
         }
 
         float acc[N][4];
@@ -449,18 +451,17 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
             const uint8_t* rec0 = smem + st * stage_bytes + kv_off;
             const int flags = stage_flags[st];
             uint32_t dep;
-            // ---- what each token multiplies by, one lane per token: f = scale s, -z f,
-            // log2 r, 1 / r, y as [page][f, z, l, ri, y][t][token 2t, 2t + 1, 2t + 8, 2t + 9]
+            // ---- what each token multiplies by, one lane per token: s (in the codes' unit),
+            // -z s, log2 r, 1 / r, y as [page][f, z, l, ri, y][t][token 2t, 2t + 1, 2t + 8, 2t + 9]
             {
                 const int tk = lane & 15;
                 const uint2 sc = *reinterpret_cast<const uint2*>(rec0 + (lane >> 4) * page_stride + kv4_scale_off(D, tk));
                 dep = sc.x;
                 const float2 ks = half2_floats(sc.x), vs = half2_floats(sc.y);
-                const float f = ks.x * 1048576.f * unit_scale;  // 2^20: the codes' unit
                 const float r = vs.x < kKv4MinScale ? kKv4MinScale : vs.x;  // keeps a NaN
                 float* dst = tokens + (lane >> 4) * 80 + ((tk & 7) >> 1) * 4 + (tk >> 3) * 2 + (tk & 1);
-                dst[0] = f;
-                dst[16] = -ks.y * f;
+                dst[0] = ks.x * 1048576.f;  // 2^20
+                dst[16] = -ks.y * ks.x;
                 dst[32] = log2_approx(r);
                 dst[48] = rcp_approx(r);
                 dst[64] = vs.y;
@@ -496,9 +497,11 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 const ulonglong2 z = *reinterpret_cast<const ulonglong2*>(tok + 16);
                 const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(tok + 32);
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    x[k2][r][0] = fma2(pair(s[0][2 * r], s[0][2 * r + 1]), f.x, fma2(z.x, qs[r], add2(l.x, minus_ref[r])));
-                    x[k2][r][1] = fma2(pair(s[1][2 * r], s[1][2 * r + 1]), f.y, fma2(z.y, qs[r], add2(l.y, minus_ref[r])));
+                for (int r = 0; r < 2; ++r) {  // a score is rounded before the reference is taken off: large ones stay in order
+                    x[k2][r][0] = fma2(pair(s[0][2 * r], s[0][2 * r + 1]), mul2(f.x, qu[r]), fma2(z.x, qs[r], l.x));
+                    x[k2][r][1] = fma2(pair(s[1][2 * r], s[1][2 * r + 1]), mul2(f.y, qu[r]), fma2(z.y, qs[r], l.y));
+                    x[k2][r][0] = add2(x[k2][r][0], minus_ref[r]);
+                    x[k2][r][1] = add2(x[k2][r][1], minus_ref[r]);
                 }
             }
             // ---- masks: a missing page, or the columns past N of the last one

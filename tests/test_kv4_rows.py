@@ -188,6 +188,54 @@ def test_graph_one_token_above_all_others(lib, heads, d):
         check_one_above(o[:, h], v, torch.full((16,), n), d)
 
 
+# --------------------------------------- query rows of very different sizes --
+
+def check_rows(q, k, v, scale, visible, got, out_dtype, rows):
+    """Each of the listed rows by itself: its tolerance comes from its own size."""
+    for r in rows:
+        want = R.attention(q[r:r + 1], k, v, scale, visible[r:r + 1])
+        R.assert_close(got[r:r + 1], want, R.tolerance(q[r:r + 1], k, v, scale, want, out_dtype), f"row {r}")
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("new,height", [(3, 8), (30, 16), (150, 128)])
+def test_attention_rows_of_very_different_sizes(lib, new, height, ratio, d):
+    """A head, and a token of the other head, far larger than the rest of the tile."""
+    context, heads = 70, 2
+    n = context + new
+    cache, bt, rows = paged([(context, new)], heads, 1, d, 5)
+    assert tile_rows(bt) == height
+    k, v = (T.randn((n, 1, d), s, torch.float16).cuda() for s in (1, 2))
+    F.store_kv4(k, v, slots_of(rows[0], n), cache, check_status=True)
+    q = T.randn((new, heads, d), 3, torch.bfloat16)
+    q[:, 0] *= ratio
+    q[1, 1] *= ratio
+    o = F.attention_kv4(q.cuda(), cache, bt, scale=d ** -0.5, out_dtype=torch.float32, check_status=True)
+    k, v = values(cache, rows[0], n)
+    visible = torch.arange(n)[None, :] <= (context + torch.arange(new))[:, None]
+    check_rows(q[:, 1].double(), k, v, d ** -0.5, visible, o[:, 1].cpu(), torch.float32, [r for r in range(new) if r != 1])
+    assert float(o.abs().max()) <= 1.01 * float(v.abs().max())  # the large ones: an average all the same
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads,d", [(1, 1, 64), (2, 1, 64), (4, 4, 64), (4, 2, 128)])
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100])
+def test_graph_rows_of_very_different_sizes(lib, heads, kv_heads, d, ratio):
+    n = 512
+    fmt = star(n)
+    cache = T.filled_cache(fmt.num_row_windows, kv_heads, d, 4)
+    q = T.randn((n, heads, d), 3, torch.bfloat16)
+    q[[3, 8, 13]] *= ratio
+    o = F.fused3s_forward_kv4(q.cuda(), cache, fmt, scale=d ** -0.5, check_status=True)
+    for h in range(heads):
+        k, v = values(cache, list(range(n // 16)), n, h // (heads // kv_heads))
+        check_rows(q[:16, h].double(), k, v, d ** -0.5, torch.ones(16, n, dtype=torch.bool), o[:16, h].cpu(), torch.float32,
+                   [r for r in range(16) if r not in (3, 8, 13)])
+        assert float(o[:16, h].abs().max()) <= 1.01 * float(v.abs().max())
+
+
 # ----------------------------------------------- scores beyond whole steps --
 
 @gpu
