@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
         // ---- Q as fp16 times a power of two that brings the row's largest to
         // [2^9, 2^10); channels whose codes come in units of 2^-24 another 2^4.
         // Lane (g, t): channels t * D / 4 ... of its rows
-        uint64_t qs[2], qu[2];  // per row, twice: scale times the sum of q; what a score's unit stands for
+        uint64_t qs[2], qu[2];  // per row, twice: the sum of q, scaled; what a score's unit stands for
         {
             uint4 raw[2][W];
             uint32_t top[2] = {0, 0};
@@ -428,8 +428,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 qsm[2 * w * 32 + lane] = make_uint4(h[0], h[4], h[1], h[5]);
                 qsm[(2 * w + 1) * 32 + lane] = make_uint4(h[2], h[6], h[3], h[7]);
             }
-            qs[0] = mul2(qu[0], pair(sum[0], sum[0]));
-            qs[1] = mul2(qu[1], pair(sum[2], sum[2]));
+            qs[0] = pair(sum[0], sum[0]);
+            qs[1] = pair(sum[2], sum[2]);
         }
 
         float acc[N][4];
@@ -498,8 +498,8 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
                 const ulonglong2 l = *reinterpret_cast<const ulonglong2*>(tok + 32);
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {  // a score is rounded before the reference is taken off: large ones stay in order
-                    x[k2][r][0] = fma2(pair(s[0][2 * r], s[0][2 * r + 1]), mul2(f.x, qu[r]), fma2(z.x, qs[r], l.x));
-                    x[k2][r][1] = fma2(pair(s[1][2 * r], s[1][2 * r + 1]), mul2(f.y, qu[r]), fma2(z.y, qs[r], l.y));
+                    x[k2][r][0] = fma2(fma2(pair(s[0][2 * r], s[0][2 * r + 1]), f.x, mul2(z.x, qs[r])), qu[r], l.x);
+                    x[k2][r][1] = fma2(fma2(pair(s[1][2 * r], s[1][2 * r + 1]), f.y, mul2(z.y, qs[r])), qu[r], l.y);
                     x[k2][r][0] = add2(x[k2][r][0], minus_ref[r]);
                     x[k2][r][1] = add2(x[k2][r][1], minus_ref[r]);
                 }
