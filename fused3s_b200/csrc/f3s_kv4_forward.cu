@@ -727,7 +727,9 @@ static int window_launch(const WindowParams& p, int64_t units, cudaStream_t stre
         return F3S_SUCCESS;
     });
     if (rc != F3S_SUCCESS) return rc;
-    const int64_t grid = std::min<int64_t>(units, C::MIN_CTAS * num_sms_of_current_device());
+    // f3s_set_forward_sm_limit counts blocks: a few of them, spread over the SMs, leave room on each
+    const int sms = num_sms_of_current_device(), limit = forward_grid_limit();
+    const int64_t grid = std::min<int64_t>(units, limit < sms ? limit : C::MIN_CTAS * sms);
     return launch_after(k_window_attend4<D, PRECISE>, (unsigned)grid, kAttendThreads,
                         p.hg < kConsumers ? C::SMEM_SHARED : C::SMEM, stream, p);
 }

@@ -65,7 +65,9 @@ int f3s_last_cuda_error(void);
  * from now on (0: one per SM, the default).  The fused kernel holds one CTA
  * per SM for its whole run; a caller that overlaps it with another kernel
  * -- an NCCL collective on a second stream, say -- leaves that kernel SMs
- * this way.  No reference counterpart. */
+ * this way.  f3s_kv4_forward, whose blocks are a third or a quarter of an SM,
+ * launches at most max_ctas of them where max_ctas is below the number of SMs.
+ * No reference counterpart. */
 int f3s_set_forward_sm_limit(int32_t max_ctas);
 
 /* ------------------------------------------------------------------------

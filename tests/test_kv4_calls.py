@@ -155,3 +155,30 @@ def test_block_tables_in_place(lib, heads, kv_heads):
         assert st == 0 and lib.f3s_workspace_status(plan.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
         got = (offsets.tolist(), positions.tolist(), slots.tolist(), table.tolist(), word.item())
         assert got == want
+
+
+@gpu
+def test_graph_forward_keeps_to_the_sm_limit(lib):
+    """Few blocks give the same result and take many times as long as all of them."""
+    n, heads, d = 40000, 4, 64
+    _, fmt = T.graph_case(n, heads, d, 5, edges=400000)
+    cache = T.filled_cache(fmt.num_row_windows, heads, d, 4)
+    order = F.generate_balanced_window_order(fmt)
+    q = T.randn((n, heads, d), 5, torch.float16).cuda()
+
+    def run():
+        out = F.fused3s_forward_kv4(q, cache, fmt, order=order, scale=0.125, check_status=True)
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        F.fused3s_forward_kv4(q, cache, fmt, order=order, scale=0.125, out=out)
+        b.record()
+        torch.cuda.synchronize()
+        return out, a.elapsed_time(b)
+
+    want, all_of_them = run()
+    try:
+        F.set_forward_sm_limit(8)
+        got, eight = run()
+    finally:
+        F.set_forward_sm_limit(0)
+    assert torch.equal(got, want) and eight > 4 * all_of_them
