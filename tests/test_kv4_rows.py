@@ -260,3 +260,73 @@ def test_attention_scores_too_large_for_fp32s_whole_steps(lib, ratio, d):
         want = R.attention(q[:, 1].double(), k, v, d ** -0.5, visible)
         R.assert_close(o[:, 1], want, R.tolerance(q[:, 1].double(), k, v, d ** -0.5, want, out_dtype))
         assert float(o.abs().max()) <= 1.01 * float(v.abs().max())
+
+
+# ------------------------------------------------------- tiles of 16 rows --
+
+SIXTEEN = [(20, 33), (0, 25), (33, 31)]  # with two query heads to a K/V head: 59 rows per request
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_16_row_tiles_leave_out_what_is_masked(lib, d):
+    assert tile_rows(paged(SIXTEEN, 4, 2, d, 1, tokens=92)[1]) == 16
+    T.test_attention_leaves_out_what_is_masked(lib, SIXTEEN, 4, d)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,height", [(1, 8), (30, 16), (150, 128)])
+def test_rising_scores_in_every_tile(lib, new, height, d):
+    lengths, n = [(800, new)], 800 + new
+    cache, bt, rows = paged(lengths, 2, 1, d, 3)
+    assert tile_rows(bt) == height
+    k = torch.ones(n, 1, d) * (torch.arange(n) / 100.0)[:, None, None]
+    F.store_kv4(k.half().cuda(), T.randn((n, 1, d), 2).half().cuda(), slots_of(rows[0], n), cache)
+    q = torch.ones(new, 2, d, dtype=torch.float16, device="cuda")
+    for out_dtype in (torch.float32, torch.bfloat16):
+        o = F.attention_kv4(q, cache, bt, scale=0.5, out_dtype=out_dtype, check_status=True)
+        want, pk, pv = T.want_attention(q, cache, rows, lengths, 0.5, 2)
+        R.assert_close(o, want, R.tolerance(q.double().cpu(), pk, pv, 0.5, want, out_dtype))
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e-4, 300.0])
+def test_extreme_sizes_in_16_row_tiles(lib, size, d):
+    tables, free, begin, num_pages = T.make_tables(SIXTEEN, 7)
+    cache = T.filled_cache(num_pages, 2, d, 5, size)
+    q = T.randn((89, 4, d), 8, torch.bfloat16, 1.0 / max(size, 1.0)).cuda()
+    bt = T.build(SIXTEEN, tables, free, begin, 89, heads=4, kv_heads=2)
+    assert tile_rows(bt) == 16
+    o = F.attention_kv4(q, cache, bt, scale=0.5, out_dtype=torch.float32, check_status=True)
+    want, pk, pv = T.want_attention(q, cache, bt.tables.tolist(), SIXTEEN, 0.5, 4)
+    R.assert_close(o, want, R.tolerance(q.double().cpu(), pk, pv, 0.5, want, torch.float32))
+    for _ in range(5):
+        assert torch.equal(F.attention_kv4(q, cache, bt, scale=0.5, out_dtype=torch.float32), o)
+
+
+@gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("new,height", [(4, 8), (20, 16), (100, 128)])
+def test_nan_reaches_only_who_sees_it_in_every_tile(lib, new, height, d):
+    cache, bt, rows = paged([(20, new)], 2, 1, d, 12)
+    assert tile_rows(bt) == height
+    n = 20 + new
+    k, v = (T.randn((n, 1, d), s, torch.float16) for s in (1, 2))
+    v[22] = math.nan
+    F.store_kv4(k.cuda(), v.cuda(), slots_of(rows[0], n), cache)
+    q = T.randn((new, 2, d), 4, torch.float16).cuda()
+    for out_dtype in (torch.float32, torch.bfloat16):
+        o = F.attention_kv4(q, cache, bt, scale=0.1, out_dtype=out_dtype)
+        assert torch.isfinite(o[:2]).all() and torch.isnan(o[2:]).all()
+    q[1, 1, 5] = math.nan
+    o = F.attention_kv4(q, cache, bt, scale=0.1, out_dtype=torch.float32)
+    assert torch.isfinite(o[0]).all() and torch.isfinite(o[1, 0]).all() and torch.isnan(o[1, 1]).all()
+
+
+@gpu
+def test_16_row_tiles_on_two_streams(lib):
+    lengths = [(700, 12), (90, 20), (0, 9)]
+    assert tile_rows(paged(lengths, 8, 2, 128, 1)[1]) == 16
+    T.test_calls_on_two_streams_share_tables_and_cache(lib, lengths)
