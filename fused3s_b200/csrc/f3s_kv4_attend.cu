@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const float z = c < 2 ? ka.y : kb.y;
-                    x[k][nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], s[nt][c]), (c < 2 ? fa : fb) * qu[nt][c & 1], c < 2 ? la : lb);
+                    x[k][nt][c] = fmaf(fmaf(-z, qs[nt][c & 1], s[nt][c]) * (c < 2 ? fa : fb), qu[nt][c & 1], c < 2 ? la : lb);
                 }
         }
         // ---- masks: only where a page has tokens that some row must not see

@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 }
             }
             const int e = amax > 0.f ? (int)(__float_as_uint(amax) >> 23) - 127 : 9;
-            const int up = min(max(9 - e, -100), 120);  // 2^(9 - floor(log2 amax)), within fp32's normal range
+            const int up = min(max(9 - e, -120), 120);  // 2^(9 - floor(log2 amax)), within fp32's normal range
             const float f = __uint_as_float((uint32_t)(up + 127) << 23);
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
@@ -162,8 +162,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 *reinterpret_cast<uint4*>(smem + C::Q + (c / 8) * (kTileRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) =
                     make_uint4(h[0], h[1], h[2], h[3]);
             }
-            rows[r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23) * 1048576.f;  // 2^20: the codes' unit
-            rows[kTileRows + r] = sum * 9.5367431640625e-7f;                              // 2^-20
+            rows[r] = p.scale * __uint_as_float((uint32_t)(127 - up) << 23);
+            rows[kTileRows + r] = sum * 9.5367431640625e-7f;  // 2^-20: the codes' unit
             fence_proxy_async_shared();
             mbar_arrive(q_full);
         }
@@ -208,8 +208,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                     // scale s (q . u - z sum(q)) + log2 r
                     uint64_t x[2] = {pair(__uint_as_float(s[4 * c]), __uint_as_float(s[4 * c + 1])),
                                      pair(__uint_as_float(s[4 * c + 2]), __uint_as_float(s[4 * c + 3]))};
-                    x[0] = fma2(mul2(f.x, scale2), fma2(z.x, qs2, x[0]), l.x);
-                    x[1] = fma2(mul2(f.y, scale2), fma2(z.y, qs2, x[1]), l.y);
+                    x[0] = fma2(mul2(f.x, fma2(z.x, qs2, x[0])), scale2, l.x);
+                    x[1] = fma2(mul2(f.y, fma2(z.y, qs2, x[1])), scale2, l.y);
                     if constexpr (HIDES) {
                         // a hidden token's scale and zero may be anything, NaN too
                         const int left = limit - (tok0 + 4 * c);  // tokens up to this one are seen
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 const float r = v2.x < kKv4MinScale ? kKv4MinScale : v2.x;  // keeps a NaN
                 // tokens that no row of the tile sees weigh nothing, whatever is there
                 const bool hidden = id < 0 || (it.page0 + 4 * j + dw) * 16 + lane > last_seen;
-                tokens[0] = hidden ? 0.f : k2.x;
+                tokens[0] = hidden ? 0.f : k2.x * 1048576.f;  // 2^20
                 tokens[64] = hidden ? 0.f : -k2.y;
                 tokens[128] = hidden ? -INFINITY : log2_approx(r);
                 tokens[192] = hidden ? 0.f : rcp_approx(r);

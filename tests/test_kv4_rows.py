@@ -199,7 +199,7 @@ def check_rows(q, k, v, scale, visible, got, out_dtype, rows):
 
 @gpu
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100, 2.0 ** 118])
 @pytest.mark.parametrize("new,height", [(3, 8), (30, 16), (150, 128)])
 def test_attention_rows_of_very_different_sizes(lib, new, height, ratio, d):
     """A head, and a token of the other head, far larger than the rest of the tile."""
@@ -221,7 +221,7 @@ def test_attention_rows_of_very_different_sizes(lib, new, height, ratio, d):
 
 @gpu
 @pytest.mark.parametrize("heads,kv_heads,d", [(1, 1, 64), (2, 1, 64), (4, 4, 64), (4, 2, 128)])
-@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100, 2.0 ** 118])
 def test_graph_rows_of_very_different_sizes(lib, heads, kv_heads, d, ratio):
     n = 512
     fmt = star(n)
@@ -240,7 +240,7 @@ def test_graph_rows_of_very_different_sizes(lib, heads, kv_heads, d, ratio):
 
 @gpu
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100])
+@pytest.mark.parametrize("ratio", [2.0 ** 30, 2.0 ** 100, 2.0 ** 118])
 def test_attention_scores_too_large_for_fp32s_whole_steps(lib, ratio, d):
     """Scores whose steps in fp32 are larger than the reach of a weight, in 128-row
     tiles: the reference settles all the same, the other rows are right, and what the
