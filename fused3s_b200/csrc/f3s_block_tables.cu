@@ -33,7 +33,7 @@ struct BlockTablesParams {
     int64_t num_tokens;
     int heads, kv_heads, group, tile_rows;
     int target;  // 0: no plan
-    int items_cap, splits_cap, slots_cap;
+    int items_cap, splits_cap, slots_cap, run_places;
     int* query_offsets;
     int* positions;
     int* slots;
@@ -319,6 +319,8 @@ __global__ void __launch_bounds__(kBtThreads) k_block_tables(const BlockTablesPa
         p.plan->kv_heads = p.kv_heads;
         p.plan->num_requests = p.requests;
         p.plan->num_tokens = (int)p.num_tokens;
+        p.plan->run_places = p.run_places;
+        for (uint32_t& w : p.plan->run_taken) w = 0;
     }
 }
 
@@ -393,6 +395,7 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
         p.items_cap = (int)L.items_cap;
         p.splits_cap = (int)L.splits_cap;
         p.slots_cap = (int)L.slots_cap;
+        p.run_places = f3s::kv4_run_places(f3s::num_sms_of_current_device());
         p.items = reinterpret_cast<f3s::Kv4Item*>(base + L.items);
         p.splits = reinterpret_cast<f3s::Kv4Split*>(base + L.splits);
         units = std::max(units, L.items_cap);

@@ -37,7 +37,10 @@ struct AttendCfg {
     static constexpr int DATA = RING > MERGE ? RING : (MERGE + 127) / 128 * 128;
     static constexpr int BARS = DATA;
     static constexpr int SINK = BARS + kAttendWarps * STAGES * 8;  // one word per warp, written, never read
-    static constexpr int SMEM = SINK + kAttendWarps * 4;
+    // sums of the runs that ended, [nt][D / 16][lane] x 4, and their references, [nt][lane] x 2, per warp
+    static constexpr int RUNS = (SINK + kAttendWarps * 4 + 15) / 16 * 16;
+    static constexpr int RUN_BYTES = NT * (D / 16) * 32 * 16 + NT * 32 * 8;
+    static constexpr int SMEM = RUNS + kAttendWarps * RUN_BYTES;
     static constexpr int MIN_CTAS = NT == 2 && D == 128 ? 3 : 4;
 };
 
@@ -231,10 +234,40 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
             den[nt][i] = off[nt][i] = 0.f;
         }
     }
+    // The sums of the runs of steps that ended, in the references as they stand; `first`: none has yet
+    auto add_runs = [&](bool first, bool keep) {
+        float4* runs = reinterpret_cast<float4*>(smem + C::RUNS + warp * C::RUN_BYTES) + lane;
+        float2* refs = reinterpret_cast<float2*>(smem + C::RUNS + warp * C::RUN_BYTES + NT * (D / 16) * 32 * 16) + lane;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float2 by = make_float2(0.f, 0.f);
+            if (!first) by = refs[32 * nt];
+            by.x = exp2_approx(by.x - ref[nt][0]);
+            by.y = exp2_approx(by.y - ref[nt][1]);
+            if (keep) refs[32 * nt] = make_float2(ref[nt][0], ref[nt][1]);
+#pragma unroll
+            for (int e = 0; e < D / 16; ++e) {
+                float(&a)[4] = acc[nt][e];
+                if (!first) {
+                    const float4 y = runs[32 * (nt * (D / 16) + e)];
+                    a[0] = fmaf(y.x, by.x, a[0]);
+                    a[1] = fmaf(y.y, by.y, a[1]);
+                    a[2] = fmaf(y.z, by.x, a[2]);
+                    a[3] = fmaf(y.w, by.y, a[3]);
+                }
+                if (keep) {
+                    runs[32 * (nt * (D / 16) + e)] = make_float4(a[0], a[1], a[2], a[3]);
+                    a[0] = a[1] = a[2] = a[3] = 0.f;
+                }
+            }
+        }
+    };
+    constexpr int RUN = kRunPages / PP;
     // first token that some row of the tile must not see
     const int open = it.context + it.row0 / p.group + 1;
 
     for (int i = 0; i < steps; ++i) {
+        if (i > 0 && i % RUN == 0) add_runs(i == RUN, true);
         const uint32_t st = i % STAGES, parity = i / STAGES & 1;
         bool ready = mbar_try_wait(bars + 8 * st, parity);
         if (!__all_sync(0xffffffffu, ready)) {
@@ -410,6 +443,8 @@ __global__ void __launch_bounds__(kAttendWarps * 32, AttendCfg<D, NT>::MIN_CTAS)
         }
     }
 
+    if (steps > RUN) add_runs(false, false);
+
     // ---- sums over the tokens of the other lanes; units of the accumulators
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -526,6 +561,18 @@ static int attend_launch(const AttendParams& p, int head_dim, int64_t units, cud
 
 }  // namespace f3s
 
+namespace f3s {
+
+// Scratch: the places of 128-row tiles' runs, then the sums of split tiles.
+static size_t run_bytes(const Kv4PlanLayout& L, int head_dim) {
+    return L.tile_rows == 128 ? (size_t)kv4_run_places(num_sms_of_current_device()) * kv4_run_floats(head_dim) * 4 : 0;
+}
+static size_t attend_scratch(const Kv4PlanLayout& L, int kv_heads, int head_dim) {
+    return run_bytes(L, head_dim) + (size_t)L.slots_cap * kv_heads * L.tile_rows * (head_dim + 2) * 4;
+}
+
+}  // namespace f3s
+
 extern "C" {
 
 size_t f3s_kv4_attention_scratch_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
@@ -534,7 +581,7 @@ size_t f3s_kv4_attention_scratch_size(int32_t num_requests, int64_t num_tokens, 
     if (head_dim != 64 && head_dim != 128) return 0;
     const f3s::Kv4PlanLayout L = f3s::kv4_plan_layout(num_requests, num_tokens, heads, kv_heads,
                                                       f3s::num_sms_of_current_device());
-    return (size_t)L.slots_cap * kv_heads * L.tile_rows * (head_dim + 2) * 4;
+    return f3s::attend_scratch(L, kv_heads, head_dim);
 }
 
 int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, int64_t q_head_stride,
@@ -555,7 +602,7 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     const f3s::Kv4PlanLayout L = f3s::kv4_plan_layout(num_requests, num_tokens, heads, kv_heads,
                                                       f3s::num_sms_of_current_device());
     if (L.items_cap > INT32_MAX / 4) return F3S_ERR_TOO_LARGE;
-    if (scratch_bytes < (size_t)L.slots_cap * kv_heads * L.tile_rows * (head_dim + 2) * 4) return F3S_ERR_WORKSPACE;
+    if (scratch_bytes < f3s::attend_scratch(L, kv_heads, head_dim)) return F3S_ERR_WORKSPACE;
     f3s::AttendParams p{};
     p.q = d_Q;
     p.q_token = q_token_stride;
@@ -571,7 +618,7 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
     p.o_dtype = o_dtype;
     p.plan = static_cast<const f3s::Kv4PlanHeader*>(d_plan);
     p.status = &static_cast<f3s::WsHeader*>(d_plan)->status;
-    p.partials = static_cast<float*>(d_scratch);
+    p.partials = reinterpret_cast<float*>(static_cast<char*>(d_scratch) + f3s::run_bytes(L, head_dim));
     p.items_cap = (int)L.items_cap;
     p.num_requests = num_requests;
     p.num_tokens = (int)num_tokens;

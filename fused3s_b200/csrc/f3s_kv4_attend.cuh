@@ -21,7 +21,7 @@ struct AttendParams {
     int o_dtype;
     int num_tokens;
     int* status;
-    float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head
+    float* partials;  // (rows of a tile) x (D + 2) floats per slot and K/V head; before it the places of runs
     const Kv4PlanHeader* plan;
     const int* tables;
     int64_t table_stride;

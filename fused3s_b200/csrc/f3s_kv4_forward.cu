@@ -62,6 +62,7 @@ struct WindowParams {
     int num_items, extra_cap, splits_cap;
     const int* cols;
     int num_nodes, windows, q_window_base, q_rows;
+    float4* runs;  // (D / 8 + 1) x 32 per consumer warp of the grid: sums of the runs that ended, references
 };
 
 // Pieces of at most `piece` blocks: half of a thread block's even share of the
@@ -72,7 +73,8 @@ struct WindowParams {
 struct WindowPieceLayout {
     int piece;
     int64_t extra_cap, splits_cap, slots_cap;
-    size_t items, splits, partials, total;
+    int64_t ctas;  // most blocks of a launch
+    size_t items, splits, partials, runs, total;
 };
 
 // Query heads to a block: 4, 2 or 1, as the counts divide.  With at most 1, 2 and 4 of
@@ -83,6 +85,9 @@ static int window_head_group(int heads, int group) {
         if (heads % hg == 0 && (group % hg == 0 || hg % group == 0)) return hg;
     return 1;
 }
+
+// Blocks that fit an SM; by head_dim (WindowCfg).
+constexpr int window_ctas(int d) { return d == 64 ? 4 : 3; }
 
 static WindowPieceLayout window_piece_layout(int num_items, int64_t num_blocks, int heads, int group, int head_dim, int sms) {
     WindowPieceLayout L{};
@@ -101,6 +106,9 @@ static WindowPieceLayout window_piece_layout(int num_items, int64_t num_blocks, 
     off += (size_t)L.splits_cap * 16;
     L.partials = off;
     off += (size_t)L.slots_cap * heads * 16 * (head_dim + 2) * 4;
+    L.ctas = std::min<int64_t>((num_items + L.extra_cap) * (heads / hg), (int64_t)window_ctas(head_dim) * sms);
+    L.runs = off;
+    off += (size_t)L.ctas * kConsumers * (head_dim / 8 + 1) * 32 * 16;
     L.total = off;
     return L;
 }
@@ -189,7 +197,7 @@ struct WindowCfg {
     static constexpr int MERGE_WORDS = ACC + 8;         // per lane
     static constexpr int SMEM = MERGE;
     static constexpr int SMEM_SHARED = MERGE + 2 * 32 * MERGE_WORDS * 4;
-    static constexpr int MIN_CTAS = D == 64 ? 4 : 3;
+    static constexpr int MIN_CTAS = window_ctas(D);
 };
 
 struct Unit {  // as the producer hands it to the consumers
@@ -441,8 +449,34 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
 #pragma unroll
         for (int r = 0; r < 2; ++r) minus_ref[r] = den[r] = off[r] = 0;
         uint32_t unset = 3;  // rows that have no reference yet (a bit each)
+        // The sums of the runs of steps that ended, in the references as they stand; `first`: none has yet
+        auto add_runs = [&](bool first, bool keep) {
+            float4* runs = p.runs + ((int64_t)blockIdx.x * kConsumers + warp) * ((N + 1) * 32) + lane;
+            const float now[2] = {unpair(minus_ref[0]).x, unpair(minus_ref[1]).x};
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (!first) y = runs[32 * N];
+            // references only rise; a row that had none has nothing to scale
+            const float by[2] = {exp2_approx(fminf(now[0] - y.x, 0.f)), exp2_approx(fminf(now[1] - y.y, 0.f))};
+            if (keep) runs[32 * N] = make_float4(now[0], now[1], 0.f, 0.f);
+#pragma unroll
+            for (int m = 0; m < N; ++m) {
+                y = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!first) y = runs[32 * m];
+                acc[m][0] = fmaf(y.x, by[0], acc[m][0]);
+                acc[m][1] = fmaf(y.y, by[0], acc[m][1]);
+                acc[m][2] = fmaf(y.z, by[1], acc[m][2]);
+                acc[m][3] = fmaf(y.w, by[1], acc[m][3]);
+                if (keep) {
+                    runs[32 * m] = make_float4(acc[m][0], acc[m][1], acc[m][2], acc[m][3]);
+                    acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+                }
+            }
+        };
+        constexpr int RUN = kRunPages / PP;  // steps of a warp in a row
 
         for (int j = turn; j < u.steps && !dead; j += turns) {
+            const int mine = j >> (turns >> 1);  // steps of this warp so far
+            if (mine > 0 && mine % RUN == 0) add_runs(mine == RUN, true);
             const uint32_t n = done + j, st = n & (p.stages - 1);
             if (!phase_wait(full + 8 * st, n / p.stages & 1, p.status, stop)) {
                 dead = true;
@@ -625,6 +659,7 @@ __global__ void __launch_bounds__(kAttendThreads, WindowCfg<D>::MIN_CTAS) k_wind
             if (lane == 0) mbar_arrive_after(empty + 8 * st, sink, dep);
         }
         done += u.steps;
+        if (u.steps - turn > RUN * turns) add_runs(false, false);
 
         // ---- per row of this lane: R, and the sums over its tokens
         float ref[2], row_den[2], row_off[2];
@@ -728,7 +763,7 @@ static int window_launch(const WindowParams& p, int64_t units, cudaStream_t stre
     });
     if (rc != F3S_SUCCESS) return rc;
     // f3s_set_forward_sm_limit counts blocks: a few of them, spread over the SMs, leave room on each
-    const int sms = num_sms_of_current_device(), limit = forward_grid_limit();
+    const int sms = num_sms_of_current_device(), limit = forward_grid_limit();  // at most the layout's ctas
     const int64_t grid = std::min<int64_t>(units, limit < sms ? limit : C::MIN_CTAS * sms);
     return launch_after(k_window_attend4<D, PRECISE>, (unsigned)grid, kAttendThreads,
                         p.hg < kConsumers ? C::SMEM_SHARED : C::SMEM, stream, p);
@@ -816,6 +851,7 @@ int f3s_kv4_forward(const void* d_Q, int32_t q_dtype, const void* d_pages, int32
     p.extra_cap = w.extra_cap;
     p.splits_cap = w.splits_cap;
     p.partials = reinterpret_cast<float*>(base + L.partials);
+    p.runs = reinterpret_cast<float4*>(base + L.runs);
     cudaStream_t s = (cudaStream_t)stream;
     F3S_CUDA_TRY(cudaMemsetAsync(base, 0, sizeof(f3s::WindowPieces), s));
     f3s::k_window_pieces<<<(unsigned)((num_items + 255) / 256), 256, 0, s>>>(w);

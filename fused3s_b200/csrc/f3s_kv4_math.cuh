@@ -22,6 +22,11 @@ namespace f3s {
 constexpr uint64_t kAttendTimeoutNs = 5ull * 1000 * 1000 * 1000;
 constexpr uint64_t kDrainNs = 100ull * 1000 * 1000;
 constexpr float kNoReference = -3.0e38f;  // finite: a weight against it is 0, not NaN
+// The tensor cores truncate when they add a product to an accumulator, and sums of codes
+// never cancel: n pages in a row lose about n 2^-25 of V's span (twice that with a
+// second product: 1.5e-2 for 250,000 pages).  After so many pages an accumulator is
+// added to a sum in fp32, rounded to nearest, and begins anew.
+constexpr int kRunPages = 256;
 constexpr float kRescaleAt = 15.f;  // log2 of the largest weight that a reference is kept for, below fp16's end
 constexpr float kTopWeight = 7.f;   // and of the largest weight when a reference is set
 

@@ -1,6 +1,7 @@
 // f3s_kv4_plan.cuh -- the attention plan that f3s_block_tables writes and
 // f3s_kv4_attention reads.
 #pragma once
+#include <algorithm>
 #include <cstdint>
 #include "f3s_internal.cuh"
 
@@ -15,7 +16,11 @@ struct Kv4PlanHeader {
     int num_items, num_splits;
     int items_cap, tile_rows;
     int heads, kv_heads, num_requests, num_tokens;  // what the plan was made with
-    int pad[56];
+    // Places in an attention's scratch for the runs of 128-row tiles, one bit each while a
+    // block of whichever attention has it; as many as blocks can run at a time.
+    int run_places;
+    uint32_t run_taken[10];
+    int pad[45];
 };
 static_assert(sizeof(Kv4PlanHeader) == 512, "plan header is 512 bytes");
 
@@ -55,6 +60,10 @@ constexpr int kKv4LongPiecePages = 64;
 __device__ __forceinline__ int kv4_parts(int pages, int piece) {
     return max((pages + (piece == kKv4MinPiecePages ? piece - 1 : piece / 2)) / piece, 1);
 }
+
+// Two blocks of 128-row tiles per SM, each with half of the tensor memory.
+inline int kv4_run_places(int sms) { return std::min(2 * sms, 10 * 32); }
+__host__ __device__ constexpr int64_t kv4_run_floats(int head_dim) { return 128 * (head_dim + 2); }
 
 struct Kv4PlanLayout {
     int tile_rows;

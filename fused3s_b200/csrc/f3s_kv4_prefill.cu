@@ -58,6 +58,28 @@ struct TileCfg {
     static constexpr int TMEM_COLUMNS = 256;         // S 2 x 64, O D
 };
 
+// A place for the sums of a block's runs, and its return; by one thread.  -1: none is
+// free, which two blocks per SM leave no room for; the accumulators then run on.
+__device__ __noinline__ int take_run_place(const Kv4PlanHeader* plan) {
+    uint32_t* taken = const_cast<uint32_t*>(plan->run_taken);
+    const int places = min(plan->run_places, 10 * 32), words = (places + 31) / 32;
+    for (int i = 0; i < 64 * words; ++i) {
+        const int w = (int)((blockIdx.x + i) % words);
+        const uint32_t all = places - 32 * w >= 32 ? 0xffffffffu : (1u << (places - 32 * w)) - 1;
+        const uint32_t free = ~(uint32_t)load_volatile(reinterpret_cast<int*>(taken + w)) & all;
+        if (free == 0) continue;
+        const uint32_t bit = free & (0u - free);
+        if (atomicOr(taken + w, bit) & bit) continue;
+        __threadfence();  // what its last owner wrote there comes first
+        return 32 * w + __ffs((int)bit) - 1;
+    }
+    return -1;
+}
+__device__ __forceinline__ void return_run_place(const Kv4PlanHeader* plan, int place) {
+    __threadfence();
+    atomicAnd(const_cast<uint32_t*>(plan->run_taken) + place / 32, ~(1u << (place % 32)));
+}
+
 template <int D, bool PRECISE>
 __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendParams p) {
     using C = TileCfg<D>;
@@ -103,6 +125,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         it.slot = b.w;
     }
     const int steps = live ? (max(it.page1 - it.page0, 0) + 3) / 4 : 0;
+    constexpr int RUN = kRunPages / 4;  // steps in a row
+    volatile int* run_place = reinterpret_cast<int*>(smem + C::TMEM_SLOT) + 1;
+    if (steps > RUN) {
+        if (threadIdx.x == 0) *run_place = take_run_place(p.plan);
+        __syncthreads();
+    }
     const int last_row = min(it.row0 + kTileRows, it.rows) - 1;
     bool ok = true;  // false: a wait ran out; the warp stops waiting
 
@@ -184,6 +212,29 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 break;
             }
             tc_fence_after();
+            if (j > 0 && j % RUN == 0 && *run_place >= 0) {  // the run ends: O, once its products are in it, goes to the sums
+                ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status, p.status) && ok;
+                tc_fence_after();
+                float* runs = p.partials - (*run_place + 1) * kv4_run_floats(D) + r;
+                const float by = j == RUN ? 0.f : exp2_approx(fminf(minus_ref - runs[(D + half) * kTileRows], 0.f));
+                runs[(D + half) * kTileRows] = minus_ref;
+#pragma unroll 1
+                for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+                    uint32_t o[32];
+                    tmem_load32(mine + 128 + c, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        float* sum = runs + (c + i) * kTileRows;
+                        const float before = j == RUN ? 0.f : *sum;
+                        *sum = fmaf(before, by, __uint_as_float(o[i]));
+                        o[i] = 0;
+                    }
+                    __syncwarp();
+                    tmem_store32(mine + 128 + c, o);
+                }
+                tc_wait_st();
+            }
             const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES) + 32 * half;
             const int tok0 = (it.page0 + 4 * j) * 16 + 32 * half;
             uint32_t hi[16], lo[PRECISE ? 16 : 1];  // P, two tokens each, and what its rounding drops
@@ -311,6 +362,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
                 tc_wait_ld();
             }
             if (!valid) continue;
+            if (steps > RUN && *run_place >= 0) {  // and the runs that ended
+                const float* runs = p.partials - (*run_place + 1) * kv4_run_floats(D) + r;
+                const float by = exp2_approx(fminf(minus_ref - runs[(D + half) * kTileRows], 0.f));
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(fmaf(runs[(c + i) * kTileRows], by, __uint_as_float(o[i])));
+            }
             // column c + 8 i + g holds channel g * D / 8 + c / 8 + i, its codes in units of
             // 2^-24 (even i) and 2^-20
 #pragma unroll
@@ -439,6 +496,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
         if (last) mbar_drain(last, last_parity, kDrainNs);
     }
     __syncthreads();
+    if (steps > RUN && threadIdx.x == 0 && *run_place >= 0) return_run_place(p.plan, *run_place);
     if (warp == kRowWarps + kCodeWarps) {
         tc_fence_after();
         tmem_free(tmem, C::TMEM_COLUMNS);

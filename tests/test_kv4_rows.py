@@ -262,6 +262,95 @@ def test_attention_scores_too_large_for_fp32s_whole_steps(lib, ratio, d):
         assert float(o.abs().max()) <= 1.01 * float(v.abs().max())
 
 
+# ---------------------------------------------------------- very long sums --
+
+def long_cache(num_pages, kv_heads, d, seed):
+    """V of +1 and -1, whose sums cancel where sums of their codes do not; and K, V in 64 bits."""
+    n = num_pages * 16
+    k = (T.randn((n, kv_heads, d), seed) * 0.3).half().cuda()
+    v = torch.where(T.randn((n, kv_heads, d), seed + 1) > 0, 1.0, -1.0).half().cuda()
+    cache = F.empty_kv4_cache(num_pages, kv_heads, d)
+    slots = torch.arange(n, dtype=torch.int32, device="cuda")
+    F.store_kv4(k, v, slots, cache, check_status=True)
+    return (cache, *(x.double() for x in F.load_kv4(cache, slots, torch.float32)))
+
+
+def check_long(got, q, k, v, scale, counts, out_dtype):
+    """got [d] of a row q [d] that sees token t of K, V [n, d] counts[t] times.
+
+    An accumulator takes at most 256 pages, two products each, before it is added to a
+    sum in fp32; an addition cuts off at most 2^-23 of the accumulator, and the
+    accumulators of a row add up to V's span, 2, at most: 512 * 2^-23 * 2.  Scores as
+    in kv4_ref.tolerance.  A lane adds up to 2^16 numbers in fp32, rounded to
+    nearest (0.29 steps of 2^-23 each, of a sum that grows): six deviations of that are
+    6 * 2^8 * 0.29 / 3^0.5 steps, in the zeros' sum and in the weights'."""
+    w = counts * torch.exp((k @ q) * scale)
+    want = (w @ v) / w.sum()
+    a = 3.0 * scale * float(q.abs().sum()) * float(k.abs().max())
+    rel = 2 * a * (k.shape[1] / 16 + 4) * 2.0 ** -22 + 64 * 2.0 ** -23 + 2 * 6 * 2.0 ** 8 * 0.29 / 3 ** 0.5 * 2.0 ** -23
+    if out_dtype == torch.bfloat16:
+        rel += 2 * 2.0 ** -11 * float(want.abs().max())  # the weights' own rounding, of their average
+    tol = 512 * 2.0 ** -23 * 2 + 2 * rel + HALF_STEP[out_dtype] * want.abs()
+    R.assert_close(got, want.cpu(), tol.cpu())
+
+
+@gpu
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("requests,new,heads,kv_heads,d,height", [
+    (64, 1, 8, 8, 64, 8), (64, 1, 8, 8, 128, 8), (8, 12, 32, 8, 64, 16), (8, 12, 32, 8, 128, 16),
+    (1, 2048, 8, 8, 64, 128), (1, 2048, 8, 8, 128, 128)])
+def test_attention_over_a_million_tokens(lib, requests, new, heads, kv_heads, d, height, out_dtype):
+    """Tables that list 512 pages again and again, 65,536 entries long."""
+    pool, repeats = 512, 128
+    tokens = pool * 16
+    cache, k, v = long_cache(pool, kv_heads, d, 5)
+    order = torch.randperm(pool, generator=T.gen(6)).int()
+    tables = order.repeat(requests, repeats).cuda()
+    context = pool * repeats * 16 - new
+    bt = F.build_block_tables(T.i32([context] * requests), T.i32([new] * requests), tables, tables[0, -new // 16 - 1:].contiguous(),
+                              None, requests * new, heads=heads, kv_heads=kv_heads)
+    assert tile_rows(bt) == height
+    tables.copy_(order.repeat(requests, repeats))  # the new pages are the pool's last again
+    q = (T.randn((requests * new, heads, d), 7) * 0.1).bfloat16().cuda()
+    o = F.attention_kv4(q, cache, bt, scale=d ** -0.5, out_dtype=out_dtype)
+    assert torch.equal(F.attention_kv4(q, cache, bt, scale=d ** -0.5, out_dtype=out_dtype), o)
+    at = (order.long()[:, None] * 16 + torch.arange(16)).reshape(-1).cuda()  # tokens of the pool, as the tables list them
+    for row, h in ((0, 0), (new - 1, heads - 1), (new // 2, 1), (requests * new - 1, 2)):
+        hidden = new - 1 - row % new  # new tokens that come later
+        counts = torch.full((tokens,), float(repeats), dtype=torch.float64, device="cuda")
+        if hidden:
+            counts[at[tokens - hidden:]] -= 1
+        g = h // (heads // kv_heads)
+        check_long(o[row, h], q[row, h].double(), k[:, g], v[:, g], d ** -0.5, counts, out_dtype)
+
+
+@gpu
+@pytest.mark.parametrize("heads,kv_heads,d", [(1, 1, 64), (2, 1, 128), (4, 1, 64), (4, 4, 64), (4, 2, 128)])
+def test_graph_window_of_very_many_blocks(lib, heads, kv_heads, d):
+    """A window of 32,000 blocks in one piece (the caller's estimate of the blocks sets its length)."""
+    blocks = 32000
+    n = blocks * 16
+    cache, k, v = long_cache(blocks, kv_heads, d, 5)
+    offsets = T.i32([0, blocks] + [blocks] * (blocks - 1))
+    cols, order = torch.arange(blocks, dtype=torch.int32, device="cuda"), T.i32([0])
+    q = (T.randn((16, heads, d), 7) * 0.1).half().cuda()
+    estimate = 900 * blocks
+    size = lib.f3s_kv4_forward_scratch_size(1, estimate, heads, kv_heads, d)
+    scratch = torch.full((size,), 0xff, dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(256, dtype=torch.uint8, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    for out_dtype, code in ((torch.float32, _lib.F3S_OUT_F32), (torch.bfloat16, _lib.F3S_OUT_BF16)):
+        o = torch.empty((16, heads, d), dtype=out_dtype, device="cuda")
+        st = lib.f3s_kv4_forward(q.data_ptr(), _lib.F3S_OUT_F16, cache.pages.data_ptr(), cache.num_pages, o.data_ptr(), code,
+                                 offsets.data_ptr(), cols.data_ptr(), order.data_ptr(), 1, estimate, n, heads, kv_heads, d,
+                                 d ** -0.5, 0, 16, ws.data_ptr(), 256, scratch.data_ptr(), size, stream)
+        assert st == 0 and lib.f3s_workspace_status(ws.data_ptr(), stream) == 0
+        for row, h in ((0, 0), (9, heads - 1), (15, heads // 2)):
+            g = h // (heads // kv_heads)
+            check_long(o[row, h], q[row, h].double(), k[:, g], v[:, g], d ** -0.5,
+                       torch.ones(n, dtype=torch.float64, device="cuda"), out_dtype)
+
+
 # ------------------------------------------------------- tiles of 16 rows --
 
 SIXTEEN = [(20, 33), (0, 25), (33, 31)]  # with two query heads to a K/V head: 59 rows per request
