@@ -80,6 +80,30 @@ __device__ __forceinline__ void return_run_place(const Kv4PlanHeader* plan, int 
     atomicAnd(const_cast<uint32_t*>(plan->run_taken) + place / 32, ~(1u << (place % 32)));
 }
 
+// Adds half of a row's columns of O to the sums of the runs before (row stride
+// kTileRows, its reference behind them) and zeroes them, by a whole warp.
+template <int D>
+__device__ __noinline__ void end_run(float* runs, uint32_t tmem_row, int half, float minus_ref, bool first) {
+    const float by = first ? 0.f : exp2_approx(fminf(minus_ref - runs[(D + half) * kTileRows], 0.f));
+    runs[(D + half) * kTileRows] = minus_ref;
+#pragma unroll 1
+    for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+        uint32_t o[32];
+        tmem_load32(tmem_row + c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            float* sum = runs + (c + i) * kTileRows;
+            const float before = first ? 0.f : *sum;
+            *sum = fmaf(before, by, __uint_as_float(o[i]));
+            o[i] = 0;
+        }
+        __syncwarp();
+        tmem_store32(tmem_row + c, o);
+    }
+    tc_wait_st();
+}
+
 template <int D, bool PRECISE>
 __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendParams p) {
     using C = TileCfg<D>;
@@ -215,25 +239,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) k_attend4_tiles(const AttendP
             if (j > 0 && j % RUN == 0 && *run_place >= 0) {  // the run ends: O, once its products are in it, goes to the sums
                 ok = phase_wait(kv_empty + 8 * (b ^ 1), (j - 1) >> 1 & 1, p.status, p.status) && ok;
                 tc_fence_after();
-                float* runs = p.partials - (*run_place + 1) * kv4_run_floats(D) + r;
-                const float by = j == RUN ? 0.f : exp2_approx(fminf(minus_ref - runs[(D + half) * kTileRows], 0.f));
-                runs[(D + half) * kTileRows] = minus_ref;
-#pragma unroll 1
-                for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
-                    uint32_t o[32];
-                    tmem_load32(mine + 128 + c, o);
-                    tc_wait_ld();
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        float* sum = runs + (c + i) * kTileRows;
-                        const float before = j == RUN ? 0.f : *sum;
-                        *sum = fmaf(before, by, __uint_as_float(o[i]));
-                        o[i] = 0;
-                    }
-                    __syncwarp();
-                    tmem_store32(mine + 128 + c, o);
-                }
-                tc_wait_st();
+                end_run<D>(p.partials - (*run_place + 1) * kv4_run_floats(D) + r, mine + 128, half, minus_ref, j == RUN);
             }
             const float* tokens = reinterpret_cast<const float*>(smem + C::TOKENS + b * C::TOKEN_BYTES) + 32 * half;
             const int tok0 = (it.page0 + 4 * j) * 16 + 32 * half;
