@@ -11,12 +11,16 @@
 // S^T = K Q^T and O^T = V^T P^T run on mma.m16n8k16 with the cache as the 16-row
 // operand (unpacked in registers, one AND per two values, f3s_kv4.cuh) and 8 NT
 // query rows as columns; P goes from accumulator to operand layout through
-// movmatrix.  tcgen05's M = 64 / 128 rows would stand mostly empty: 4 to 16 query
-// rows share a page.
+// movmatrix.  (With eight pages as the 128 rows of a tcgen05 product the queries would
+// fill its columns just as well, but the codes would have to be unpacked into shared
+// memory first; that form has not been built or measured for so few query rows.)
+//
+// Accumulators are emptied every kRunPages pages (f3s_kv4_math.cuh) into sums that lie
+// in shared memory beside the ring.
 //
 // Bound: HBM and instruction issue together.  64 requests of up to 8,191 tokens, one
-// new token each, 32 / 8 heads, D = 128: 351 MB in 76 us, 4.6 TB/s (the copies
-// alone take 59 us; issue slots 55 % busy, most of it unpacking and weights).
+// new token each, 32 / 8 heads, D = 128, bf16: 351 MB in 79 us, 4.4 TB/s (issue slots
+// 57 % busy, most of it unpacking and weights; the copies alone took 59 us).
 //
 #include <algorithm>
 #include "f3s_kv4_attend.cuh"

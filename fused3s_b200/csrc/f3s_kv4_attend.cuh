@@ -5,8 +5,8 @@
 
 namespace f3s {
 
-// No field more than fits: with 24 bytes of parameters more, the kernel of 128-row
-// tiles got other registers and took 271 us instead of 255.
+// The kernel of 128-row tiles sits at its register limit (72, a few of them spilled), so
+// its time moves by some percent with small changes anywhere, these fields among them.
 struct AttendParams {
     const void* q;
     int64_t q_token, q_head;  // strides in elements

@@ -15,13 +15,20 @@
 // of S are the operand registers of P.  What a token multiplies by (scale, zero,
 // log2 r, 1 / r, y) is worked out by one lane per token, put down in shared memory
 // and read as pairs; the arithmetic on scores runs on pairs of fp32 numbers.
-// tcgen05's M = 64 / 128 rows would stand mostly empty at 16 rows per window.
+// (tcgen05 with the queries as rows would be an eighth full; with eight pages as its 128
+// rows it would need the codes unpacked into shared memory, which has not been built or
+// measured here.)
 //
-// Bound: instruction issue (56 % of the slots, mma.sync 43 %), since each window
-// unpacks its pages for itself.  131,057 nodes of 8 heads, D = 64, 22 blocks per window
-// (94 GFLOP, 508 MB from HBM, fp16 O): 632 us; the copies alone take 219 us.  40,009
-// nodes of 4 / 2 heads, D = 128, 80 blocks per window (105 GFLOP, 92 % of
-// the pages from L2, bf16 O): 455 us.
+// Accumulators are emptied every kRunPages pages (f3s_kv4_math.cuh) into sums in scratch,
+// a place per consumer warp of the grid.
+//
+// 131,057 nodes of 8 heads, D = 64, 22 blocks per window (94 GFLOP, 516 MB from HBM, fp16
+// O): 666 us; the copies alone took 219 us, and the products, half as many again for fp16
+// O, need 267 us at the 530 TFLOP/s that mma.sync reaches.  40,009 nodes of 4 / 2 heads, D = 128, 80
+// blocks per window (105 GFLOP, 85 % of the pages from L2, bf16 O): 454 us.  No unit is
+// full: issue slots 56 and 51 % busy, mma.sync 40 and 45 %.  Each warp goes through score, vote,
+// weight and product one after another, unpacks its pages and works out the tokens'
+// numbers for itself, and spills (64 to 164 bytes a thread).
 //
 #include <algorithm>
 #include "f3s_kv4_math.cuh"
@@ -78,8 +85,8 @@ struct WindowPieceLayout {
 };
 
 // Query heads to a block: 4, 2 or 1, as the counts divide.  With at most 1, 2 and 4 of
-// 8 heads 1,075, 800 and 632 us (131,057 nodes, d = 64), of 4 / 2 heads 599, 533 and 455 (40,009
-// nodes, d = 128); 2,708 nodes of 8 heads, d = 64, 56, 51 and 60.
+// 8 heads 1,164, 866 and 657 us (131,057 nodes, d = 64), of 4 / 2 heads 552, 482 and 447 (40,009
+// nodes, d = 128); 2,708 nodes of 8 heads, d = 64, 58, 54 and 62.
 static int window_head_group(int heads, int group) {
     for (int hg = 4; hg > 1; hg >>= 1)
         if (heads % hg == 0 && (group % hg == 0 || hg % group == 0)) return hg;

@@ -83,13 +83,18 @@ inline Kv4PlanLayout kv4_plan_layout(int num_requests, int64_t num_tokens, int h
     const int64_t mean = num_requests > 0 ? (rows + num_requests - 1) / num_requests : 0;
     // Rows per request -> us with tiles of 8, 16, 128 rows (64 requests of 1,024 tokens,
     // 8 K/V heads, D = 128; 64 requests, 2 K/V heads, D = 64; 8 requests, 8 heads, D = 128):
-    //   24:  51, 55, 103
-    //   32:                16, 27, 47    21, 25, 48
-    //   48:  92, 79, 107
-    //   64: 120, 99, 108   26, 21, 37    21, 35, 56
-    //   96: 176, 143, 115  37, 31, 39
-    //  128: 232, 189, 123  46, 35, 41    34, 35, 56
-    //  256:                86, 65, 44    63, 54, 55
+    //   24:  51, 60,  94   16, 27, 46   17, 25, 45
+    //   32:  64, 59,  96   16, 28, 47   21, 26, 46
+    //   48:  92, 85,  99   23, 21, 34   21, 32, 52
+    //   64: 120, 106, 101  26, 22, 37   21, 37, 54
+    //   96: 176, 153, 108  37, 32, 39   30, 36, 49
+    //  128: 232, 202, 116  46, 36, 41   34, 38, 53
+    //  256: 458, 393, 223  87, 66, 42   63, 58, 52
+    // The rule looks at the mean alone: where few requests leave SMs idle, lower tiles are
+    // faster than what it takes (8 requests of 64 rows: 21 against 37 us), and a batch
+    // of unequal requests gets one height for all (63 decoding requests and a prompt of
+    // 2,000 tokens: 178 us, 21 and 95 apart), as does one with spare capacity (64 decoding
+    // requests in a batch for 2,048 tokens: 93 us).
     // Tiles of 32 rows on mma.sync were never faster than the best of these.
     L.tile_rows = mean <= 32 ? 8 : mean <= 96 ? 16 : 128;
     const int64_t tiles = rows / L.tile_rows + num_requests;

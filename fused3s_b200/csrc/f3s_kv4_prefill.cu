@@ -20,11 +20,15 @@
 // V's rows are ordered so that unpacking does not collide in shared memory's
 // banks: row r holds channel (r % 8) * D / 8 + r / 8.
 //
-// Bound: the weights (13 instructions and 2.5 loads from shared memory per two
-// scores; issue slots 39 % busy), then the products (128 x 64 x D twice per step;
-// tensor pipe 16 %).  Five prompts of up to 3,200 tokens, 32 / 8 heads, D = 128, 81
-// GFLOP: 255 us, 319 TFLOP/s.  With one thread per row and 64 tokens each 316 us;
-// mma.sync with 32 rows 506.
+// Accumulators are emptied every kRunPages pages (f3s_kv4_math.cuh) into sums in
+// scratch, in a place that a block with more pages than that takes for its run.
+//
+// Bound: a chain of short waits (scores, vote, weights, product) with neither unit
+// full: issue slots 44 % busy, most of it the weights (15 instructions and 2.5 loads from
+// shared memory per two scores), tensor pipe 16 %.  Five prompts of up to 3,200 tokens,
+// 32 / 8 heads, D = 128, 81 GFLOP, in a CUDA graph: 245 us with bf16 results, 332 TFLOP/s;
+// 267 with fp16 and 273 with fp32 ones.  When it was first built, one thread per row
+// with 64 tokens each took 316 us against 255, mma.sync with 32 rows 506.
 #include <algorithm>
 #include <type_traits>
 #include "f3s_kv4_attend.cuh"

@@ -500,8 +500,12 @@ int f3s_block_tables(const int32_t* d_context_lens, const int32_t* d_new_lens, i
  *            shared by calls that may overlap; needs no initialisation
  * A table entry of -1 holds no tokens (they are left out); one outside the
  * cache is too, and is reported as F3S_ERR_BAD_FORMAT in the plan's status.
- * fp16 and fp32 O are exact to fp32 arithmetic, bf16 O rounds the softmax
- * weights to fp16.
+ * Sums are held in fp32, with products added to accumulators for at most 256 pages
+ * in a row (such a run loses some 1e-5 of V's span to the tensor cores' truncation).
+ * For fp16 and fp32 O a softmax weight is multiplied in two fp16 parts, 2^-21 of it or
+ * 2^-32 of the row's largest; for bf16 O it is rounded to fp16, the same in every sum.
+ * Exponentials, logarithms and reciprocals are the hardware's approximations, a few
+ * units of 2^-23.
  * ---------------------------------------------------------------------- */
 size_t f3s_kv4_attention_scratch_size(int32_t num_requests, int64_t num_tokens, int32_t heads, int32_t kv_heads,
                                         int32_t head_dim);
@@ -520,8 +524,9 @@ int f3s_kv4_attention(const void* d_Q, int32_t q_dtype, int64_t q_token_stride, 
  * num_blocks (the active blocks of the listed windows, or an estimate) sets how
  * heavy windows are cut into pieces for several SMs, merged in order, so no plan
  * is needed; it does not change which blocks are computed.  d_workspace
- * (f3s_forward_workspace_size bytes, zeroed once) keeps the status; d_scratch: f3s_kv4_forward_scratch_size bytes, 16-byte
- * aligned, not shared by calls that may overlap, needs no initialisation.
+ * (f3s_forward_workspace_size bytes, zeroed once) keeps the status; d_scratch:
+ * f3s_kv4_forward_scratch_size bytes, 16-byte aligned, not shared by calls that may
+ * overlap, needs no initialisation.  Arithmetic as in f3s_kv4_attention.
  * ---------------------------------------------------------------------- */
 size_t f3s_kv4_forward_scratch_size(int32_t num_items, int64_t num_blocks, int32_t heads, int32_t kv_heads,
                                     int32_t head_dim);
