@@ -91,9 +91,11 @@ constexpr float kWhole = 12582912.f;
 // in the low half of code[i], 2i + 1 in the high one.  Scale and zero are the
 // row's, in each of its 8 lanes.
 //
-// x / s is computed as q + (x - q s) / s with q = x * (1 / s): the residual is
-// exact, so the result is exact where it is a half-integer and off by 1 ulp at
-// most elsewhere, and rounding it to a whole number is right.
+// x / s is computed as q + (x - q s) / s with q = x * (1 / s), a quotient corrected by
+// its residual (P. Markstein, Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990): the residual is exact in a fused multiply-add, so
+// the result is exact where it is a half-integer and off by 1 ulp at most elsewhere,
+// and rounding it to a whole number is right.
 template <class T, int CH>
 __device__ __forceinline__ void quantise(const uint32_t (&raw)[CH / 2], uint32_t (&code)[CH / 2], __half& scale, float& zero) {
     uint32_t lo2 = 0, hi2 = 0;
